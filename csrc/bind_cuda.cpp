@@ -15,6 +15,8 @@ std::vector<at::Tensor> layernorm_fwd_fp8(const at::Tensor& x, const at::Tensor&
 at::Tensor layernorm_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& gamma,
                          const at::Tensor& mean, const at::Tensor& rstd, at::Tensor dgamma,
                          at::Tensor dbeta, bool accumulate, const c10::optional<at::Tensor>& dres);
+// decoder_ops.cpp
+void bind_decoder_ops(pybind11::module& m);
 // xent.cu
 at::Tensor xent_fused(at::Tensor logits, const at::Tensor& targets,
                       const c10::optional<at::Tensor>& grad_scale, double scale_mul,
@@ -173,6 +175,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("grad_scale") = py::none(), py::arg("scale_mul") = 1.0,
         py::arg("write_grad") = true, py::arg("out8") = py::none(), py::arg("out8_scale") = py::none(),
         py::arg("out8_amax") = py::none());
+  bind_decoder_ops(m);
   m.def("optim_grad_sumsq", &optim_grad_sumsq);
   m.def("optim_finalize", &optim_finalize);
   m.def("adam_step", &adam_step);

@@ -447,6 +447,21 @@ class GptModel(nn.Module):
         return LMHeadLossFn.apply(h, targets, (self.lm_head.weight, self.lm_head.bias), grad_scale,
                                   self._head_fp8())
 
+    @torch.no_grad()
+    def fused_token_logprobs(self, input_ids: torch.Tensor, targets: torch.Tensor, *, temperature: float = 1.0,
+                             top: int = 0, entropy: bool = False):
+        """Scores given continuations through the fused kernels: for each position the log
+        probability of its target (a target outside the vocabulary is ignored), and on request
+        the entropy and the ``top`` likeliest tokens (``mtorus.ops.logprobs.TokenLogprobs``,
+        [B, S] each).  bf16 LM head; records no gradient."""
+        from ..ops import kernels as K
+        from ..ops.logprobs import token_logprobs
+
+        h = self.fused_hidden(input_ids)
+        logits = K.gemm(h, self.lm_head.weight.w16, bias=self.lm_head.bias.data)
+        return token_logprobs(logits.view(*targets.shape, self.vocab_size), targets, temperature=temperature, top=top,
+                              entropy=entropy)
+
     def _head_fp8(self):
         """The FP8 state when the LM head runs in FP8, else None."""
         return getattr(self, "fp8_state", None) if getattr(self, "fp8_head", False) else None

@@ -18,6 +18,7 @@ from typing import Optional, Tuple
 import torch
 
 from .._ext import cuda as _cuda
+from .rotary import RotaryPositions, rotary_, rotary_qkv
 
 HEAD_DIM = 128
 TILE = 128
@@ -69,22 +70,37 @@ def attention_bwd(dout: torch.Tensor, qkv: torch.Tensor, out: torch.Tensor, lse:
 
 class CausalAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, B, S, H):
+    def forward(ctx, qkv, B, S, H, rope=None, positions=None):
+        if rope is not None:
+            qkv = rotary_qkv(qkv, B, S, H, rope, positions)
         out, lse = attention_fwd(qkv, B, S, H)
-        ctx.save_for_backward(qkv, out, lse)
-        ctx.dims = (B, S, H)
+        ctx.save_for_backward(qkv, out, lse, positions)
+        ctx.dims, ctx.rope = (B, S, H), rope
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        qkv, out, lse = ctx.saved_tensors
-        return attention_bwd(dout, qkv, out, lse, *ctx.dims), None, None, None
+        qkv, out, lse, positions = ctx.saved_tensors
+        B, S, H = ctx.dims
+        dqkv = attention_bwd(dout, qkv, out, lse, B, S, H)
+        if ctx.rope is not None:  # dq and dk turn back where they lie
+            heads = dqkv.view(B, S, 3 * H, HEAD_DIM)
+            rotary_(heads[:, :, :H], heads[:, :, H:2 * H], ctx.rope, positions, inverse=True)
+        return dqkv, None, None, None, None, None
 
 
-def causal_attention(qkv: torch.Tensor, B: int, S: int, H: int, dh: int) -> torch.Tensor:
-    """qkv: [B*S, 3*H*dh] bf16 (q | k | v, heads contiguous) -> [B*S, H*dh]."""
+def causal_attention(qkv: torch.Tensor, B: int, S: int, H: int, dh: int, rotary: Optional[RotaryPositions] = None,
+                     positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qkv: [B*S, 3*H*dh] bf16 (q | k | v, heads contiguous) -> [B*S, H*dh].
+    rotary: rotary positions on q and k (``mtorus.ops.rotary``), at ``positions`` ([S] or [B, S];
+    default 0 .. S-1); their gradient is turned back in place."""
     check_shape(S, dh)
-    return CausalAttentionFn.apply(qkv, B, S, H)
+    if rotary is None:
+        if positions is not None:
+            raise ValueError("positions without rotary")
+        return CausalAttentionFn.apply(qkv, B, S, H)
+    rotary._check(dh)
+    return CausalAttentionFn.apply(qkv, B, S, H, rotary, positions)
 
 
 def reference_attention(qkv: torch.Tensor, B: int, S: int, H: int, dh: int,

@@ -36,7 +36,8 @@ host_sources = _rel(
 ) + ["csrc/bind_host.cpp"]
 
 cuda_sources = _rel(glob.glob(os.path.join(ROOT, "csrc/kernels/*.cu"))) + [
-    "csrc/bind_cuda.cpp"
+    "csrc/bind_cuda.cpp",
+    "csrc/decoder_ops.cpp",
 ]
 
 common_cxx = ["-O3", "-std=c++17", "-Wno-unused-function"]
