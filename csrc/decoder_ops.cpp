@@ -50,6 +50,14 @@ at::Tensor rows_of(const at::Tensor& t) {
 at::Tensor or_undefined(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
+bool needs_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts) {
+    if (t->defined() && t->requires_grad()) return true;
+  }
+  return false;
+}
+
 void no_double_backward(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the gradient has no gradient (backward with create_graph=True)");
 }
@@ -172,7 +180,13 @@ std::tuple<at::Tensor, OptTensor> rotary(const at::Tensor& q, const OptTensor& k
   const at::Tensor qt = tokens_of(q), kt = or_undefined(k);
   const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1));
   check_cuda({&q, &kt, &turns, pos.has_value() ? &*pos : &turns}, "rotary");
-  auto out = RotaryFn::apply(q, k, turns, pos, rot_dim, interleaved, scale, offset, q.size(-2));
+  variable_list out;
+  if (needs_grad({&q, &kt}))
+    out = RotaryFn::apply(q, k, turns, pos, rot_dim, interleaved, scale, offset, q.size(-2));
+  else if (kt.defined())
+    out = rotary_raw({q, kt}, r, pos, offset, false, {q.size(-2), kt.size(-2)});
+  else
+    out = rotary_raw({q}, r, pos, offset, false, {q.size(-2)});
   return {out[0], k.has_value() ? OptTensor(out[1]) : c10::nullopt};
 }
 
@@ -189,7 +203,9 @@ at::Tensor rotary_qkv(const at::Tensor& qkv, int64_t B, int64_t S, int64_t heads
   check_rotary(x, "qkv", r);
   const OptTensor pos = positions_of(positions, B, S);
   check_cuda({&qkv, &turns, pos.has_value() ? &*pos : &turns}, "rotary_qkv");
-  auto out = RotaryFn::apply(x, OptTensor(), turns, pos, rot_dim, interleaved, scale, offset, heads + kv_heads);
+  const auto out = needs_grad({&x}) ? RotaryFn::apply(x, OptTensor(), turns, pos, rot_dim, interleaved, scale, offset,
+                                                      heads + kv_heads)
+                                    : rotary_raw({x}, r, pos, offset, false, {heads + kv_heads});
   return out[0].view(qkv.sizes());
 }
 
@@ -263,6 +279,32 @@ ResidualNormArgs norm_args(const at::Tensor& x, const at::Tensor& h, const at::T
   return a;
 }
 
+struct NormOutputs {
+  at::Tensor y, n, rstd_h, rstd_y;
+  variable_list list() const {
+    variable_list out;
+    if (y.defined()) out.push_back(y);
+    if (n.defined()) out.push_back(n);
+    return out;
+  }
+};
+
+NormOutputs norm_forward(const at::Tensor& x, const at::Tensor& h, const at::Tensor& pre, const at::Tensor& post,
+                         const at::Tensor& gate, int kind, double beta, double alpha, double eps, bool statistics) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const ResidualNormArgs a = norm_args(x, h, pre, post, gate, kind, beta, alpha, eps);
+  NormOutputs o;
+  if (h.defined()) o.y = at::empty(x.sizes(), x.options());
+  if (pre.defined()) o.n = at::empty(x.sizes(), x.options());
+  if (statistics) {
+    const at::Tensor stats = at::empty({2, a.x.size(0)}, x.options().dtype(at::kFloat));
+    if (post.defined()) o.rstd_h = stats.select(0, 0);
+    if (pre.defined()) o.rstd_y = stats.select(0, 1);
+  }
+  residual_norm_fwd_launch(a, o.y, o.n, o.rstd_h, o.rstd_y);
+  return o;
+}
+
 struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& branch,
                                const OptTensor& pre_weight, const OptTensor& post_weight, const OptTensor& gate_,
@@ -270,30 +312,15 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
     at::AutoDispatchBelowADInplaceOrView g;
     const at::Tensor h = or_undefined(branch), pre = or_undefined(pre_weight), post = or_undefined(post_weight),
                      gate = or_undefined(gate_);
-    c10::cuda::CUDAGuard guard(x.device());
     ctx->set_materialize_grads(false);
-    const ResidualNormArgs a = norm_args(x, h, pre, post, gate, (int)kind, beta, alpha, eps);
-    const bool grad = x.requires_grad() || (h.defined() && h.requires_grad()) ||
-                      (pre.defined() && pre.requires_grad()) || (post.defined() && post.requires_grad()) ||
-                      (gate.defined() && gate.requires_grad());
-    const int64_t rows = a.x.size(0);
-    const auto f32 = x.options().dtype(at::kFloat);
-    at::Tensor y, n, rstd_h, rstd_y;
-    if (h.defined()) y = at::empty(x.sizes(), x.options());
-    if (pre.defined()) n = at::empty(x.sizes(), x.options());
-    if (grad && post.defined()) rstd_h = at::empty({rows}, f32);
-    if (grad && pre.defined()) rstd_y = at::empty({rows}, f32);
-    residual_norm_fwd_launch(a, y, n, rstd_h, rstd_y);
-    ctx->save_for_backward({x, h, pre, post, gate, rstd_h, rstd_y});
+    const NormOutputs o = norm_forward(x, h, pre, post, gate, (int)kind, beta, alpha, eps, true);
+    ctx->save_for_backward({x, h, pre, post, gate, o.rstd_h, o.rstd_y});
     auto& d = ctx->saved_data;
     d["kind"] = kind;
     d["beta"] = beta;
     d["alpha"] = alpha;
     d["eps"] = eps;
-    variable_list out;
-    if (y.defined()) out.push_back(y);
-    if (n.defined()) out.push_back(n);
-    return out;
+    return o.list();
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -350,7 +377,10 @@ std::tuple<at::Tensor, OptTensor> residual_norm(const at::Tensor& x, const at::T
   TORCH_CHECK_VALUE(std::isfinite(residual_scale) && std::isfinite(branch_scale) && eps >= 0 && std::isfinite(eps),
                     "residual_norm: the scales must be finite and eps at least 0");
   check_cuda({&x, &branch, &pw, &qw, &gt}, "residual_norm");
-  auto out = ResidualNormFn::apply(x, OptTensor(branch), pre, post, gate, (int64_t)kind, residual_scale, branch_scale, eps);
+  const auto out =
+      needs_grad({&x, &branch, &pw, &qw, &gt})
+          ? ResidualNormFn::apply(x, OptTensor(branch), pre, post, gate, (int64_t)kind, residual_scale, branch_scale, eps)
+          : norm_forward(x, branch, pw, qw, gt, kind, residual_scale, branch_scale, eps, false).list();
   return {out[0], pw.defined() ? OptTensor(out[1]) : c10::nullopt};
 }
 
@@ -359,6 +389,8 @@ at::Tensor rms_norm(const at::Tensor& x, const at::Tensor& weight, double eps) {
   check_weight(weight, x.size(-1), "weight");
   TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "rms_norm: eps must be at least 0");
   check_cuda({&x, &weight}, "rms_norm");
+  if (!needs_grad({&x, &weight}))
+    return norm_forward(x, at::Tensor(), weight, at::Tensor(), at::Tensor(), kGateNone, 1.0, 1.0, eps, false).n;
   const OptTensor none;
   return ResidualNormFn::apply(x, none, OptTensor(weight), none, none, (int64_t)kGateNone, 1.0, 1.0, eps)[0];
 }
@@ -367,36 +399,49 @@ at::Tensor rms_norm(const at::Tensor& x, const at::Tensor& weight, double eps) {
 
 namespace {
 
+struct LogprobOutputs {
+  at::Tensor tokens, logprob, stats, entropy, top_lp, top_ids;
+  variable_list list() const {
+    variable_list out{logprob};
+    for (const at::Tensor* t : {&entropy, &top_lp, &top_ids}) {
+      if (t->defined()) out.push_back(*t);
+    }
+    return out;
+  }
+};
+
+LogprobOutputs logprobs_forward(const at::Tensor& logits, const at::Tensor& tokens, double inv_tau, int64_t top,
+                                bool entropy) {
+  c10::cuda::CUDAGuard guard(logits.device());
+  const at::Tensor x = rows_of(logits);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  LogprobOutputs o;
+  o.tokens = tokens.dim() == 1 ? tokens.contiguous() : tokens.reshape({-1}).contiguous();
+  o.logprob = at::empty(tokens.sizes(), f32);
+  o.stats = at::empty({x.size(0), 2}, f32);
+  if (entropy) o.entropy = at::empty(tokens.sizes(), f32);
+  if (top > 0) {
+    std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+    shape.push_back(top);
+    o.top_lp = at::empty(shape, f32);
+    o.top_ids = at::empty(shape, tokens.options());
+  }
+  token_logprobs_fwd_launch(x, o.tokens, inv_tau, top, o.logprob, o.stats, o.entropy, o.top_lp, o.top_ids);
+  return o;
+}
+
 struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& tokens,
                                double inv_tau, int64_t top, bool entropy) {
     at::AutoDispatchBelowADInplaceOrView g;
-    c10::cuda::CUDAGuard guard(logits.device());
     ctx->set_materialize_grads(false);
-    const at::Tensor x = rows_of(logits), t = tokens.reshape({-1}).contiguous();
-    const int64_t rows = x.size(0);
-    const auto f32 = logits.options().dtype(at::kFloat);
-    std::vector<int64_t> top_shape(tokens.sizes().begin(), tokens.sizes().end());
-    top_shape.push_back(top);
-    at::Tensor lp = at::empty(tokens.sizes(), f32), stats = at::empty({rows, 2}, f32), ent, top_lp, top_ids;
-    if (entropy) ent = at::empty(tokens.sizes(), f32);
-    if (top > 0) {
-      top_lp = at::empty(top_shape, f32);
-      top_ids = at::empty(top_shape, tokens.options());
-    }
-    token_logprobs_fwd_launch(x, t, inv_tau, top, lp, stats, ent, top_lp, top_ids);
-    ctx->save_for_backward({logits, t, stats, ent, top_ids});
+    const LogprobOutputs o = logprobs_forward(logits, tokens, inv_tau, top, entropy);
+    ctx->save_for_backward({logits, o.tokens, o.stats, o.entropy, o.top_ids});
     ctx->saved_data["inv_tau"] = inv_tau;
     ctx->saved_data["top"] = top;
     ctx->saved_data["entropy"] = entropy;
-    variable_list out{lp};
-    if (entropy) out.push_back(ent);
-    if (top > 0) {
-      ctx->mark_non_differentiable({top_ids});
-      out.push_back(top_lp);
-      out.push_back(top_ids);
-    }
-    return out;
+    if (top > 0) ctx->mark_non_differentiable({o.top_ids});
+    return o.list();
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -438,7 +483,8 @@ std::tuple<at::Tensor, OptTensor, OptTensor, OptTensor> token_logprobs(const at:
   TORCH_CHECK_VALUE(temperature >= 1e-6 && temperature <= 1e6,
                     "token_logprobs: the temperature must be from 1e-6 to 1e6, not ", temperature);
   check_cuda({&logits, &tokens}, "token_logprobs");
-  auto out = TokenLogprobsFn::apply(logits, tokens, 1.0 / temperature, top, entropy);
+  const auto out = needs_grad({&logits}) ? TokenLogprobsFn::apply(logits, tokens, 1.0 / temperature, top, entropy)
+                                         : logprobs_forward(logits, tokens, 1.0 / temperature, top, entropy).list();
   size_t at = 1;
   OptTensor ent, top_lp, top_ids;
   if (entropy) ent = out[at++];

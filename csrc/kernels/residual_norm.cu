@@ -1,16 +1,20 @@
 // Residual update of a block with its norms, in one pass each way:
 //   rh = 1/sqrt(mean h^2 + eps),  b = h rh post,   y = beta x + alpha g b     (post norm, gate, scales)
 //   ry = 1/sqrt(mean y^2 + eps),  n = y ry pre                               (pre norm of the next block)
-// Backward, with u = dn pre, yh = y ry, hh = h rh:
+// Backward, with u = dn pre, yh = y ry, hh = h rh and e = alpha g post (a gate per row stays out of e, as r):
 //   Y = dy + ry (u - yh mean(u yh));  dx = beta Y;  dg = alpha b Y;  dpre = sum dn yh;  dpost = sum alpha g Y hh
-//   dh = rh (alpha g post Y - hh mean(alpha g b Y))
+//   dh = rh (r e Y - hh mean(r e hh Y))
 // y is computed again from x and h in 32 bits (reading x instead of y costs the same bytes), so the statistics
 // and the weight gradients see the value before its rounding.
 //
 // Bound by memory: forward 2 reads and 2 writes of [T, d], backward 4 and 2.  One CTA of d / 8 threads walks a
-// strided set of rows; a thread owns the same 8 columns of every row, so the sums of weight gradients stay in its
-// registers and leave once per CTA, to be added up in a fixed order by a second kernel.  The backward needs one
-// row reduction, not two: mean(alpha g b Y) follows from sums of alpha g b with dy, u and yh.
+// strided set of rows; a thread owns the same 8 columns of every row, so the weights and the sums of weight
+// gradients stay in its registers.  Its vectors of the next rows are on their way through a ring in shared memory;
+// each thread reads back only what it copied itself, so the ring needs no barrier.
+//
+// The backward needs little more than the memory's time in instructions, so it is written to need few: one row
+// reduction, not two (mean(e hh Y) follows from sums of e hh with dy, u and yh), one column sum q = sum r Y hh for
+// both dpost = alpha g q and dgate = alpha post q, pairs of values per instruction, and 6 shuffles for 4 row sums.
 #include "decoder_ops.h"
 #include "vec.cuh"
 
@@ -19,17 +23,21 @@ namespace mtorus {
 namespace {
 
 constexpr int kMaxWarps = 32;
+constexpr int kSmemBudget = 200 * 1024;  // of 227 KB per SM: the CTAs' static part and the system's 1 KB each fit too
+
+// Tensors that are read row by row.
+enum In : int { kX = 0, kH = 1, kGate = 2, kDy = 3, kDn = 4, kIns = 5 };
 
 struct NormParams {
-  const void *x, *h, *dy, *dn, *gate;
-  int64_t ldx, ldh, lddy, lddn, ldg;
-  const float *pre, *post;
+  const void* in[kIns];  // nullptr: not there
+  int64_t ld[kIns];
+  const float *pre, *post, *gate;  // gate: per channel or per row
   void *y, *n, *dx, *dh, *dgate;
   float *rstd_h, *rstd_y, *part;
   int64_t rows;
-  int d, gate_kind;
+  int d, gate_kind, depth, stage;  // ring: rows in flight, bytes of one row's slots
   float beta, alpha, eps;
-  int want_dpre, want_dpost, want_dgate;
+  bool want_dpre, want_q;
 };
 
 // Columns of a thread's 8 values in a group of 256 columns: vectors of 16 bytes where rows are aligned
@@ -41,330 +49,453 @@ __device__ __forceinline__ int col_of(int group, int lane, int i) {
   return group * 256 + (i / VEC) * (32 * VEC) + lane * VEC + i % VEC;
 }
 
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load8(const T* row, int group, int lane, int d, float* f) {
-  if constexpr (ALIGNED) {
-    constexpr int VEC = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8; i += VEC) {
-      const int c = col_of<T, ALIGNED>(group, lane, i);
-      Vec<T, VEC> v;
-      if (c < d) v = load_stream(reinterpret_cast<const Vec<T, VEC>*>(row + c));
-      widen(v, f + i);
-      if (c >= d) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) f[i + k] = 0.f;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = col_of<T, ALIGNED>(group, lane, i);
-      f[i] = c < d ? to_f<T>(row[c]) : 0.f;
-    }
-  }
-}
-
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store8(T* row, int group, int lane, int d, const float* f) {
-  if constexpr (ALIGNED) {
-    constexpr int VEC = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8; i += VEC) {
-      const int c = col_of<T, ALIGNED>(group, lane, i);
-      if (c < d) store_stream(reinterpret_cast<Vec<T, VEC>*>(row + c), narrow<T, VEC>(f + i));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = col_of<T, ALIGNED>(group, lane, i);
-      if (c < d) row[c] = from_f<T>(f[i]);
-    }
-  }
-}
-
-// Weights are fp32 vectors of d values; missing ones read as `none`.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load_weight(const float* w, int group, int lane, int d, float none, float* f) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = col_of<T, ALIGNED>(group, lane, i);
-    f[i] = w != nullptr && c < d ? w[c] : none;
-  }
-}
-
-// Sums of N values over the CTA; every thread gets them.  `red` holds [2][kMaxWarps][N] floats and `par`
-// alternates between its halves, so one barrier per call is enough.
-template <int N>
-__device__ __forceinline__ void cta_sum(float (&v)[N], float* red, int& par) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = warp_sum(v[k]);
-  const int nw = blockDim.x >> 5;
-  if (nw == 1) return;
-  float* r = red + par * kMaxWarps * N;
-  par ^= 1;
-  if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) r[(threadIdx.x >> 5) * N + k] = v[k];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = 0.f;
-  for (int w = 0; w < nw; ++w) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] += r[w * N + k];
-  }
-}
-
+// The rows that a thread has asked for, and their values. The slots of one row lie one input after another, each
+// with one 16-byte vector of every thread after the other.
 template <typename T, bool ALIGNED, int NG>
-__global__ void __launch_bounds__(1024) residual_norm_fwd(const __grid_constant__ NormParams p) {
-  __shared__ float red[2 * kMaxWarps];
-  const int lane = threadIdx.x & 31, g0 = (threadIdx.x >> 5) * NG, d = p.d;
-  const float inv_d = 1.f / d;
-  int par = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    float x[NG][8], y[NG][8];
+struct Rows {
+  static constexpr int VEC = 16 / sizeof(T), NV = 8 / VEC;
+  const NormParams& p;
+  unsigned char* ring;
+  int lane, g0;
+
+  __device__ __forceinline__ Rows(const NormParams& p, unsigned char* ring)
+      : p(p), ring(ring), lane(threadIdx.x & 31), g0((threadIdx.x >> 5) * NG) {}
+
+  __device__ __forceinline__ unsigned char* slot(int stage, int input, int k) const {
+    int at = 0;  // inputs before this one
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      load8<T, ALIGNED>(static_cast<const T*>(p.x) + row * p.ldx, g0 + g, lane, d, x[g]);
-      if (p.h != nullptr) load8<T, ALIGNED>(static_cast<const T*>(p.h) + row * p.ldh, g0 + g, lane, d, y[g]);
-    }
-    if (p.h != nullptr) {
-      float rh = 1.f;
-      if (p.post != nullptr) {
-        float s[1] = {0.f};
+    for (int t = 0; t < kIns; ++t) at += t < input && p.in[t] != nullptr;
+    return ring + stage * p.stage + ((at * NG * NV + k) * blockDim.x + threadIdx.x) * 16;
+  }
+
+  __device__ __forceinline__ void ask(int64_t row, int stage) const {
+    if constexpr (ALIGNED) {
+      if (row < p.rows) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int t = 0; t < kIns; ++t) {
+          if (p.in[t] == nullptr) continue;
+          const T* src = static_cast<const T*>(p.in[t]) + row * p.ld[t];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) s[0] += y[g][i] * y[g][i];
-        cta_sum<1>(s, red, par);
-        rh = rsqrtf(s[0] * inv_d + p.eps);
-        if (threadIdx.x == 0 && p.rstd_h != nullptr) p.rstd_h[row] = rh;
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+              const int c = col_of<T, true>(g0 + g, lane, k * VEC);
+              copy_async16(slot(stage, t, g * NV + k), src + (c < p.d ? c : 0), c < p.d);
+            }
+        }
       }
-      float gr = p.alpha * rh;
-      if (p.gate_kind == kGateRow) gr *= static_cast<const float*>(p.gate)[row];
+      copy_async_commit();
+    }
+  }
+
+  // the 8 values of group g as pairs; 0 beyond d and where the input is not there
+  __device__ __forceinline__ void get(int input, int64_t row, int stage, int g, float2 (&f)[4]) const {
+    float v[8];
+    if (p.in[input] == nullptr) {
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float w[8];
-        if (p.post != nullptr) {
-          load_weight<T, ALIGNED>(p.post, g0 + g, lane, d, 0.f, w);
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    } else if constexpr (ALIGNED) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[g][i] *= w[i];
-        }
-        if (p.gate_kind == kGateChannel) {
-          load_weight<T, ALIGNED>(static_cast<const float*>(p.gate), g0 + g, lane, d, 0.f, w);
+      for (int k = 0; k < NV; ++k)
+        widen(*reinterpret_cast<const Vec<T, VEC>*>(slot(stage, input, g * NV + k)), v + k * VEC);
+    } else {
+      const T* src = static_cast<const T*>(p.in[input]) + row * p.ld[input];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[g][i] *= w[i];
-        }
-        if (p.gate_kind == kGateFull) {
-          load8<T, ALIGNED>(static_cast<const T*>(p.gate) + row * p.ldg, g0 + g, lane, d, w);
+      for (int i = 0; i < 8; ++i) {
+        const int c = col_of<T, false>(g0 + g, lane, i);
+        v[i] = c < p.d ? to_f<T>(src[c]) : 0.f;
+      }
+    }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[g][i] *= w[i];
-        }
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+  }
+
+  __device__ __forceinline__ void put(void* out, int64_t row, int g, const float2 (&f)[4]) const {
+    T* dst = static_cast<T*>(out) + row * p.d;
+    float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[g][i] = p.beta * x[g][i] + gr * y[g][i];
-        if (p.y != nullptr) store8<T, ALIGNED>(static_cast<T*>(p.y) + row * d, g0 + g, lane, d, y[g]);
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = f[i].x;
+      v[2 * i + 1] = f[i].y;
+    }
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = col_of<T, true>(g0 + g, lane, k * VEC);
+        if (c < p.d) store_stream(reinterpret_cast<Vec<T, VEC>*>(dst + c), narrow<T, VEC>(v + k * VEC));
       }
     } else {
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[g][i] = x[g][i];
-    }
-    if (p.n == nullptr) continue;
-    float s[1] = {0.f};
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[0] += y[g][i] * y[g][i];
-    cta_sum<1>(s, red, par);
-    const float ry = rsqrtf(s[0] * inv_d + p.eps);
-    if (threadIdx.x == 0 && p.rstd_y != nullptr) p.rstd_y[row] = ry;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float w[8];
-      load_weight<T, ALIGNED>(p.pre, g0 + g, lane, d, 0.f, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] *= y[g][i] * ry;
-      store8<T, ALIGNED>(static_cast<T*>(p.n) + row * d, g0 + g, lane, d, w);
+      for (int i = 0; i < 8; ++i) {
+        const int c = col_of<T, false>(g0 + g, lane, i);
+        if (c < p.d) dst[c] = from_f<T>(v[i]);
+      }
     }
   }
+
+  // fp32 weights [d]; `none` where there are none or beyond d
+  __device__ __forceinline__ void weight(const float* w, int g, float none, float2 (&f)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c0 = col_of<T, ALIGNED>(g0 + g, lane, 2 * i), c1 = col_of<T, ALIGNED>(g0 + g, lane, 2 * i + 1);
+      f[i].x = w != nullptr && c0 < p.d ? w[c0] : none;
+      f[i].y = w != nullptr && c1 < p.d ? w[c1] : none;
+    }
+  }
+
+  // e = alpha g post without a gate per row or per element
+  __device__ __forceinline__ void branch_weight(int g, float2 (&e)[4]) const {
+    float2 w[4];
+    weight(p.post, g, 1.f, e);
+    weight(p.gate_kind == kGateChannel ? p.gate : nullptr, g, 1.f, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = mul2(mul2(e[i], w[i]), both(p.alpha));
+  }
+};
+
+// Sum of one value over the CTA for every thread. `red` holds [2][kMaxWarps] floats; `par` alternates between its
+// halves, so that one barrier per call is enough.
+__device__ __forceinline__ float cta_sum(float v, float* red, int& par) {
+  v = warp_sum(v);
+  const int nw = blockDim.x >> 5;
+  if (nw == 1) return v;
+  float* r = red + par * kMaxWarps;
+  par ^= 1;
+  if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int w = 0; w < nw; ++w) v += r[w];
+  return v;
 }
 
-// part: [gridDim.x][3][d] sums over the CTA's rows of dpre, dpost and the per-channel dgate.
-template <typename T, bool ALIGNED, int NG>
-__global__ void __launch_bounds__(1024) residual_norm_bwd(const __grid_constant__ NormParams p) {
-  __shared__ float red[2 * kMaxWarps * 4];
-  const int lane = threadIdx.x & 31, g0 = (threadIdx.x >> 5) * NG, d = p.d;
-  const float inv_d = 1.f / d;
-  int par = 0;
-  float sum_pre[NG][8], sum_post[NG][8], sum_gate[NG][8];
+// The same for four values: the halves of the warp first share the values out among them, so that 6 shuffles do.
+__device__ __forceinline__ float4 cta_sum4(float4 v, float4* red, int& par) {
+  const int lane = threadIdx.x & 31;
+  const bool up = lane & 16, odd = lane & 8;
+  const float a = (up ? v.z : v.x) + __shfl_xor_sync(0xffffffffu, up ? v.x : v.z, 16);
+  const float b = (up ? v.w : v.y) + __shfl_xor_sync(0xffffffffu, up ? v.y : v.w, 16);
+  float s = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
 #pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum_pre[g][i] = sum_post[g][i] = sum_gate[g][i] = 0.f;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    float x[NG][8], h[NG][8], dy[NG][8], dn[NG][8];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      load8<T, ALIGNED>(static_cast<const T*>(p.x) + row * p.ldx, g0 + g, lane, d, x[g]);
-      if (p.h != nullptr) load8<T, ALIGNED>(static_cast<const T*>(p.h) + row * p.ldh, g0 + g, lane, d, h[g]);
-      if (p.dy != nullptr) load8<T, ALIGNED>(static_cast<const T*>(p.dy) + row * p.lddy, g0 + g, lane, d, dy[g]);
-      if (p.dn != nullptr) load8<T, ALIGNED>(static_cast<const T*>(p.dn) + row * p.lddn, g0 + g, lane, d, dn[g]);
-    }
-    const float rh = p.post != nullptr ? p.rstd_h[row] : 1.f;
-    const float ry = p.dn != nullptr ? p.rstd_y[row] : 0.f;
-    const float gr = p.gate_kind == kGateRow ? static_cast<const float*>(p.gate)[row] : 1.f;
-    // s: sum u yh, and sums of c = alpha (g) b with dy, u and yh; a gate per row is left out of c
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float wpre[8], wpost[8], gate[8];
-      load_weight<T, ALIGNED>(p.pre, g0 + g, lane, d, 0.f, wpre);
-      load_weight<T, ALIGNED>(p.post, g0 + g, lane, d, 1.f, wpost);
-      if (p.gate_kind == kGateFull)
-        load8<T, ALIGNED>(static_cast<const T*>(p.gate) + row * p.ldg, g0 + g, lane, d, gate);
-      else
-        load_weight<T, ALIGNED>(p.gate_kind == kGateChannel ? static_cast<const float*>(p.gate) : nullptr, g0 + g,
-                                lane, d, 1.f, gate);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (p.dy == nullptr) dy[g][i] = 0.f;
-        const float c = p.h != nullptr ? p.alpha * gate[i] * (h[g][i] * rh * wpost[i]) : 0.f;
-        const float y = p.beta * x[g][i] + gr * c;
-        x[g][i] = y * ry;  // yh
-        const float u = p.dn != nullptr ? dn[g][i] * wpre[i] : 0.f;
-        if (p.dn != nullptr) sum_pre[g][i] += dn[g][i] * x[g][i];
-        dn[g][i] = u;
-        s[0] += u * x[g][i];
-        s[1] += c * dy[g][i];
-        s[2] += c * u;
-        s[3] += c * x[g][i];
-      }
-    }
-    cta_sum<4>(s, red, par);
-    const float m = s[0] * inv_d;
-    const float cy = s[1] + ry * (s[2] - m * s[3]);  // sum c Y
-    if (p.want_dgate && p.gate_kind == kGateRow && threadIdx.x == 0) static_cast<float*>(p.dgate)[row] = cy;
-    const float k = gr * cy * inv_d;  // mean(alpha g b Y)
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float wpost[8], gate[8], o[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dy[g][i] += ry * (dn[g][i] - x[g][i] * m);  // Y
-      if (p.dx != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = p.beta * dy[g][i];
-        store8<T, ALIGNED>(static_cast<T*>(p.dx) + row * d, g0 + g, lane, d, o);
-      }
-      if (p.h == nullptr) continue;
-      load_weight<T, ALIGNED>(p.post, g0 + g, lane, d, 1.f, wpost);
-      if (p.gate_kind == kGateFull)
-        load8<T, ALIGNED>(static_cast<const T*>(p.gate) + row * p.ldg, g0 + g, lane, d, gate);
-      else
-        load_weight<T, ALIGNED>(p.gate_kind == kGateChannel ? static_cast<const float*>(p.gate) : nullptr, g0 + g,
-                                lane, d, gr, gate);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float hh = h[g][i] * rh, ay = p.alpha * dy[g][i];
-        const float db = gate[i] * ay;
-        sum_post[g][i] += db * hh;
-        const float dg = hh * wpost[i] * ay;
-        sum_gate[g][i] += dg;
-        gate[i] = dg;
-        o[i] = p.post != nullptr ? rh * (db * wpost[i] - hh * k) : db;
-      }
-      if (p.dh != nullptr) store8<T, ALIGNED>(static_cast<T*>(p.dh) + row * d, g0 + g, lane, d, o);
-      if (p.want_dgate && p.gate_kind == kGateFull)
-        store8<T, ALIGNED>(static_cast<T*>(p.dgate) + row * d, g0 + g, lane, d, gate);
-    }
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  // lanes 0, 8, 16, 24 hold the sums of x, y, z, w
+  const int nw = blockDim.x >> 5;
+  if (nw == 1) {
+    v.x = __shfl_sync(0xffffffffu, s, 0);
+    v.y = __shfl_sync(0xffffffffu, s, 8);
+    v.z = __shfl_sync(0xffffffffu, s, 16);
+    v.w = __shfl_sync(0xffffffffu, s, 24);
+    return v;
   }
+  float4* r = red + par * kMaxWarps;
+  par ^= 1;
+  if ((lane & 7) == 0) reinterpret_cast<float*>(r + (threadIdx.x >> 5))[lane >> 3] = s;
+  __syncthreads();
+  float2 lo = both(0.f), hi = both(0.f);
+  for (int w = 0; w < nw; ++w) {
+    const float4 t = r[w];
+    lo = add2(lo, make_float2(t.x, t.y));
+    hi = add2(hi, make_float2(t.z, t.w));
+  }
+  return make_float4(lo.x, lo.y, hi.x, hi.y);
+}
+
+template <typename T, bool ALIGNED, int NG, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float red[2 * kMaxWarps];
+  const Rows<T, ALIGNED, NG> in(p, ring);
+  const float inv_d = 1.f / p.d;
+  const bool branch = p.in[kH] != nullptr;
+  int par = 0, stage = 0;
+  float2 e[NG][4], pre[NG][4];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    in.branch_weight(g, e[g]);
+    in.weight(p.pre, g, 0.f, pre[g]);
+  }
+  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + (int64_t)k * gridDim.x, k);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    in.ask(row + (int64_t)(p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
+    const float gate = p.gate_kind == kGateRow ? p.gate[row] : 1.f;
+    if constexpr (ALIGNED) copy_async_wait(p.depth - 1);
+    float2 y[NG][4];
+    if (branch) {
+      float rh = 1.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) in.get(kH, row, stage, g, y[g]);
+      if (p.post != nullptr) {
+        float2 s = both(0.f);
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s = fma2(y[g][i], y[g][i], s);
+        rh = rsqrtf(cta_sum(s.x + s.y, red, par) * inv_d + p.eps);
+        if (threadIdx.x == 0 && p.rstd_h != nullptr) p.rstd_h[row] = rh;
+      }
+      const float2 r = both(rh * gate), beta = both(p.beta);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float2 x[4];
+        in.get(kX, row, stage, g, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[g][i] = mul2(y[g][i], e[g][i]);
+        if (p.gate_kind == kGateFull) {
+          float2 w[4];
+          in.get(kGate, row, stage, g, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[g][i] = mul2(y[g][i], w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[g][i] = fma2(y[g][i], r, mul2(x[i], beta));
+        in.put(p.y, row, g, y[g]);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) in.get(kX, row, stage, g, y[g]);
+    }
+    if (p.n != nullptr) {
+      float2 s = both(0.f);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fma2(y[g][i], y[g][i], s);
+      const float ry = rsqrtf(cta_sum(s.x + s.y, red, par) * inv_d + p.eps);
+      if (threadIdx.x == 0 && p.rstd_y != nullptr) p.rstd_y[row] = ry;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[g][i] = mul2(mul2(y[g][i], both(ry)), pre[g][i]);
+        in.put(p.n, row, g, y[g]);
+      }
+    }
+    stage = stage + 1 == p.depth ? 0 : stage + 1;
+  }
+  if constexpr (ALIGNED) copy_async_wait(0);
+}
+
+// part: [gridDim.x][2][d], the CTA's sums of dn yh (dpre) and of r Y hh (q; with the gate of each element)
+template <typename T, bool ALIGNED, int NG, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float4 red[2 * kMaxWarps];
+  const Rows<T, ALIGNED, NG> in(p, ring);
+  const float inv_d = 1.f / p.d;
+  const bool branch = p.in[kH] != nullptr, full = p.gate_kind == kGateFull, post = p.post != nullptr;
+  int par = 0, stage = 0;
+  float2 e[NG][4], pre[NG][4], sum_pre[NG][4], sum_q[NG][4];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    in.branch_weight(g, e[g]);
+    in.weight(p.in[kDn] != nullptr ? p.pre : nullptr, g, 0.f, pre[g]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum_pre[g][i] = sum_q[g][i] = both(0.f);
+  }
+  float next_rh = 1.f, next_ry = 0.f, next_gate = 1.f;
+  auto ask_scalars = [&](int64_t row) {
+    if (row >= p.rows) return;
+    if (post) next_rh = p.rstd_h[row];
+    if (p.in[kDn] != nullptr) next_ry = p.rstd_y[row];
+    if (p.gate_kind == kGateRow) next_gate = p.gate[row];
+  };
+  ask_scalars(blockIdx.x);
+  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + (int64_t)k * gridDim.x, k);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    in.ask(row + (int64_t)(p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
+    const float rh = next_rh, ry = next_ry, gate = next_gate;
+    ask_scalars(row + gridDim.x);
+    if constexpr (ALIGNED) copy_async_wait(p.depth - 1);
+    float2 hh[NG][4], yh[NG][4], dy[NG][4], u[NG][4];
+    // sums of u yh, and of c = e hh with dy, u and yh
+    float2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f), s3 = both(0.f);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      in.get(kX, row, stage, g, yh[g]);
+      in.get(kH, row, stage, g, hh[g]);
+      in.get(kDy, row, stage, g, dy[g]);
+      in.get(kDn, row, stage, g, u[g]);
+      float2 c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        hh[g][i] = mul2(hh[g][i], both(rh));
+        c[i] = mul2(hh[g][i], e[g][i]);
+      }
+      if (full) {
+        float2 w[4];
+        in.get(kGate, row, stage, g, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = mul2(c[i], w[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        yh[g][i] = mul2(fma2(c[i], both(gate), mul2(yh[g][i], both(p.beta))), both(ry));
+        sum_pre[g][i] = fma2(u[g][i], yh[g][i], sum_pre[g][i]);
+        u[g][i] = mul2(u[g][i], pre[g][i]);
+        s0 = fma2(u[g][i], yh[g][i], s0);
+        s1 = fma2(c[i], dy[g][i], s1);
+        s2 = fma2(c[i], u[g][i], s2);
+        s3 = fma2(c[i], yh[g][i], s3);
+      }
+    }
+    const float4 s = cta_sum4(make_float4(s0.x + s0.y, s1.x + s1.y, s2.x + s2.y, s3.x + s3.y), red, par);
+    const float m = s.x * inv_d;
+    const float cy = s.y + ry * (s.z - m * s.w);  // sum of c Y
+    if (p.gate_kind == kGateRow && p.dgate != nullptr && threadIdx.x == 0) static_cast<float*>(p.dgate)[row] = cy;
+    const float2 minus_m = both(-m), minus_k = both(-rh * gate * cy * inv_d), r = both(post ? rh * gate : gate);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float2 o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dy[g][i] = fma2(fma2(yh[g][i], minus_m, u[g][i]), both(ry), dy[g][i]);  // Y
+        o[i] = mul2(dy[g][i], both(p.beta));
+      }
+      if (p.dx != nullptr) in.put(p.dx, row, g, o);
+      if (!branch) continue;
+      if (full) {
+        float2 w[4];
+        if (p.dgate != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = mul2(mul2(hh[g][i], e[g][i]), dy[g][i]);
+          in.put(p.dgate, row, g, o);
+        }
+        in.get(kGate, row, stage, g, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dy[g][i] = mul2(dy[g][i], w[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum_q[g][i] = fma2(mul2(dy[g][i], both(gate)), hh[g][i], sum_q[g][i]);
+        o[i] = mul2(mul2(dy[g][i], e[g][i]), r);
+        if (post) o[i] = fma2(hh[g][i], minus_k, o[i]);
+      }
+      if (p.dh != nullptr) in.put(p.dh, row, g, o);
+    }
+    stage = stage + 1 == p.depth ? 0 : stage + 1;
+  }
+  if constexpr (ALIGNED) copy_async_wait(0);
   if (p.part == nullptr) return;
-  float* part = p.part + (int64_t)blockIdx.x * 3 * d;
+  float* part = p.part + (int64_t)blockIdx.x * 2 * p.d;
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = col_of<T, ALIGNED>(g0 + g, lane, i);
-      if (c >= d) continue;
-      if (p.want_dpre) part[c] = sum_pre[g][i];
-      if (p.want_dpost) part[d + c] = sum_post[g][i];
-      if (p.want_dgate && p.gate_kind == kGateChannel) part[2 * d + c] = sum_gate[g][i];
+      const int c = col_of<T, ALIGNED>(in.g0 + g, in.lane, i);
+      if (c >= p.d) continue;
+      if (p.want_dpre) part[c] = i & 1 ? sum_pre[g][i / 2].y : sum_pre[g][i / 2].x;
+      if (p.want_q) part[p.d + c] = i & 1 ? sum_q[g][i / 2].y : sum_q[g][i / 2].x;
     }
 }
 
-// Sums the CTAs' partial weight gradients in a fixed order: one CTA per 32 columns of one gradient.
-__global__ void __launch_bounds__(256) residual_norm_finish(const float* part, int parts, int d, float* dpre,
-                                                            float* dpost, float* dgate) {
-  __shared__ float sm[8][32];
-  float* out = blockIdx.y == 0 ? dpre : blockIdx.y == 1 ? dpost : dgate;
-  if (out == nullptr) return;
+// Sums the CTAs' parts in a fixed order, one CTA for 32 columns: dpre, or q and from it dpost = alpha g q and
+// dgate = alpha post q.
+constexpr int kFinishWarps = 32;
+__global__ void __launch_bounds__(kFinishWarps * 32)
+    residual_norm_finish(const float* part, int parts, int d, bool first, float alpha, const float* gate,
+                         const float* post, float* dpre, float* dpost, float* dgate) {
+  __shared__ float sm[kFinishWarps][32];
+  const bool is_pre = first && blockIdx.y == 0;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float t = 0.f;
   if (c < d) {
-    const float* col = part + (int64_t)blockIdx.y * d + c;
-#pragma unroll 8
-    for (int b = w; b < parts; b += 8) t += col[(int64_t)b * 3 * d];
+    const float* col = part + (is_pre ? 0 : d) + c;
+#pragma unroll 4
+    for (int b = w; b < parts; b += kFinishWarps) t += col[(int64_t)b * 2 * d];
   }
   sm[w][lane] = t;
   __syncthreads();
-  if (w == 0 && c < d) {
+  if (w != 0 || c >= d) return;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += sm[k][lane];
-    out[c] = t;
+  for (int k = 1; k < kFinishWarps; ++k) t += sm[k][lane];
+  if (is_pre) {
+    dpre[c] = t;
+  } else {
+    if (dpost != nullptr) dpost[c] = alpha * (gate != nullptr ? gate[c] : 1.f) * t;
+    if (dgate != nullptr) dgate[c] = alpha * (post != nullptr ? post[c] : 1.f) * t;
   }
 }
 
 struct Shape {
   bool aligned;
-  int groups, threads;
+  int threads, groups, ins;
 };
 
 // Rows are read in 16-byte vectors where every tensor's rows start on 16 bytes.
 Shape shape_of(const NormParams& p, int esize) {
-  bool ok = p.d % (16 / esize) == 0;
-  for (int64_t ld : {p.ldx, p.ldh, p.lddy, p.lddn, p.ldg}) ok = ok && ld % (16 / esize) == 0;
-  for (const void* q : {p.x, p.h, p.dy, p.dn, (const void*)p.y, (const void*)p.n, (const void*)p.dx,
-                        (const void*)p.dh})
-    ok = ok && reinterpret_cast<uintptr_t>(q) % 16 == 0;
-  if (p.gate_kind == kGateFull)
-    ok = ok && reinterpret_cast<uintptr_t>(p.gate) % 16 == 0 && reinterpret_cast<uintptr_t>(p.dgate) % 16 == 0;
+  const int v = 16 / esize;
+  bool ok = p.d % v == 0;
+  int ins = 0;
+  for (int t = 0; t < kIns; ++t) {
+    ok = ok && p.ld[t] % v == 0 && reinterpret_cast<uintptr_t>(p.in[t]) % 16 == 0;
+    ins += p.in[t] != nullptr;
+  }
+  for (const void* q : {p.y, p.n, p.dx, p.dh}) ok = ok && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+  if (p.gate_kind == kGateFull) ok = ok && reinterpret_cast<uintptr_t>(p.dgate) % 16 == 0;
   const int per = (p.d + 255) / 256, groups = per > kMaxWarps ? 2 : 1;
-  return Shape{ok, groups, (per + groups - 1) / groups * 32};
+  const int threads = (per + groups - 1) / groups * 32;
+  ok = ok && ins * groups * threads * 8 * esize <= kSmemBudget;  // a row has to fit into the ring
+  return Shape{ok, threads, groups, ins};
 }
 
+// f(ALIGNED, NG, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
 template <typename F>
 void with_shape(const Shape& s, F&& f) {
-  auto g = [&](auto al) {
-    if (s.groups == 1)
-      f(al, std::integral_constant<int, 1>{});
+  auto go = [&](auto al) {
+    using std::integral_constant;
+    if (s.groups == 2)
+      f(al, integral_constant<int, 2>{}, integral_constant<int, 1024>{});
+    else if (s.threads > 512)
+      f(al, integral_constant<int, 1>{}, integral_constant<int, 1024>{});
+    else if (s.threads > 256)
+      f(al, integral_constant<int, 1>{}, integral_constant<int, 512>{});
     else
-      f(al, std::integral_constant<int, 2>{});
+      f(al, integral_constant<int, 1>{}, integral_constant<int, 256>{});
   };
   if (s.aligned)
-    g(std::true_type{});
+    go(std::true_type{});
   else
-    g(std::false_type{});
+    go(std::false_type{});
+}
+
+// The ring's depth for `fit` CTAs per SM, and the CTAs that are resident with it.
+int64_t plan_ring(NormParams& p, const Shape& s, int esize, int fit, int deepest) {
+  p.depth = 1;
+  if (s.aligned) {
+    p.stage = s.ins * s.groups * s.threads * 8 * esize;
+    p.depth = std::min(deepest, std::max(1, kSmemBudget / fit / p.stage));
+    fit = std::max(1, std::min(fit, kSmemBudget / (p.stage * p.depth)));
+  }
+  return (int64_t)num_sms() * fit;
+}
+
+template <typename K>
+void launch_norm(K kernel, const NormParams& p, const Shape& s, unsigned grid) {
+  const int smem = p.stage * p.depth;
+  if (smem > 40 * 1024)  // without asking, a CTA gets 48 KB, its static part included
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget));
+  kernel<<<grid, s.threads, smem, cur_stream()>>>(p);
+  MT_LAUNCH_CHECK();
 }
 
 const void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 NormParams params_of(const ResidualNormArgs& a) {
   NormParams p{};
-  p.x = a.x.data_ptr();
+  p.in[kX] = a.x.data_ptr();
   p.rows = a.x.size(0);
   p.d = (int)a.x.size(1);
   auto ld = [](const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : int64_t(0); };
-  p.ldx = ld(a.x);
+  p.ld[kX] = ld(a.x);
   if (a.h.has_value()) {
-    p.h = a.h->data_ptr();
-    p.ldh = ld(*a.h);
+    p.in[kH] = a.h->data_ptr();
+    p.ld[kH] = ld(*a.h);
   }
   if (a.pre.has_value()) p.pre = a.pre->data_ptr<float>();
   if (a.post.has_value()) p.post = a.post->data_ptr<float>();
-  if (a.gate.has_value()) {
-    p.gate = a.gate->data_ptr();
-    if (a.gate_kind == kGateFull) p.ldg = ld(*a.gate);
+  if (a.gate_kind == kGateFull) {
+    p.in[kGate] = a.gate->data_ptr();
+    p.ld[kGate] = ld(*a.gate);
+  } else if (a.gate.has_value()) {
+    p.gate = a.gate->data_ptr<float>();
   }
   p.gate_kind = a.gate_kind;
   p.beta = (float)a.beta;
@@ -386,11 +517,11 @@ void residual_norm_fwd_launch(const ResidualNormArgs& a, const at::Tensor& y, co
   dispatch_act(a.x.scalar_type(), [&](auto t) {
     using T = decltype(t);
     const Shape s = shape_of(p, sizeof(T));
-    with_shape(s, [&](auto al, auto ng) {
-      const int64_t resident = (int64_t)num_sms() * std::max(1, 2048 / s.threads);
-      const unsigned grid = (unsigned)std::min<int64_t>(p.rows, resident);
-      residual_norm_fwd<T, decltype(al)::value, decltype(ng)::value><<<grid, s.threads, 0, cur_stream()>>>(p);
-      MT_LAUNCH_CHECK();
+    with_shape(s, [&](auto al, auto ng, auto maxt) {
+      constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 1024 ? 1 : 1024 / kMaxT;
+      const int fit = std::min(16, kMinB * kMaxT / s.threads);
+      const unsigned grid = (unsigned)std::min<int64_t>(p.rows, plan_ring(p, s, sizeof(T), fit, 4));
+      launch_norm(residual_norm_fwd<T, decltype(al)::value, decltype(ng)::value, kMaxT, kMinB>, p, s, grid);
     });
   });
 }
@@ -400,20 +531,18 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
                               const at::Tensor& dgate, const at::Tensor& dpre, const at::Tensor& dpost) {
   NormParams p = params_of(a);
   auto ld = [](const at::Tensor& t) { return t.defined() && t.size(0) > 1 ? t.stride(0) : int64_t(0); };
-  p.dy = ptr(dy);
-  p.lddy = ld(dy);
-  p.dn = ptr(dn);
-  p.lddn = ld(dn);
+  p.in[kDy] = ptr(dy);
+  p.ld[kDy] = ld(dy);
+  p.in[kDn] = ptr(dn);
+  p.ld[kDn] = ld(dn);
   p.dx = const_cast<void*>(ptr(dx));
   p.dh = const_cast<void*>(ptr(dh));
   p.dgate = const_cast<void*>(ptr(dgate));
   p.rstd_h = rstd_h.defined() ? rstd_h.data_ptr<float>() : nullptr;
   p.rstd_y = rstd_y.defined() ? rstd_y.data_ptr<float>() : nullptr;
-  p.want_dpre = dpre.defined();
-  p.want_dpost = dpost.defined();
-  p.want_dgate = dgate.defined();
   const bool gate_sum = dgate.defined() && a.gate_kind == kGateChannel;
-  const bool sums = dpre.defined() || dpost.defined() || gate_sum;
+  p.want_dpre = dpre.defined();
+  p.want_q = dpost.defined() || gate_sum;
   if (p.rows == 0) {
     for (const at::Tensor* t : {&dpre, &dpost}) {
       if (t->defined()) t->zero_();
@@ -424,20 +553,23 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
   dispatch_act(a.x.scalar_type(), [&](auto t) {
     using T = decltype(t);
     const Shape s = shape_of(p, sizeof(T));
-    with_shape(s, [&](auto al, auto ng) {
-      const int64_t resident = (int64_t)num_sms() * std::max(1, 1024 / s.threads);
-      const unsigned grid = (unsigned)std::min<int64_t>(p.rows, resident);
+    with_shape(s, [&](auto al, auto ng, auto maxt) {
+      constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 256 ? 2 : 1;
+      const int fit = std::min(16, kMinB * kMaxT / s.threads);
+      int64_t grid = std::min<int64_t>(p.rows, plan_ring(p, s, sizeof(T), fit, 4));
       at::Tensor part;
-      if (sums) {
-        part = at::empty({(int64_t)grid, 3, (int64_t)p.d}, a.x.options().dtype(at::kFloat));
+      if (p.want_dpre || p.want_q) {
+        // a few rows for each CTA at least: its partial sums cost as much as two rows
+        grid = std::min(grid, (p.rows + 3) / 4);
+        part = at::empty({grid, 2, (int64_t)p.d}, a.x.options().dtype(at::kFloat));
         p.part = part.data_ptr<float>();
       }
-      residual_norm_bwd<T, decltype(al)::value, decltype(ng)::value><<<grid, s.threads, 0, cur_stream()>>>(p);
-      MT_LAUNCH_CHECK();
-      if (sums) {
-        residual_norm_finish<<<dim3((p.d + 31) / 32, 3), 256, 0, cur_stream()>>>(
-            p.part, (int)grid, p.d, dpre.defined() ? dpre.data_ptr<float>() : nullptr,
-            dpost.defined() ? dpost.data_ptr<float>() : nullptr, gate_sum ? dgate.data_ptr<float>() : nullptr);
+      launch_norm(residual_norm_bwd<T, decltype(al)::value, decltype(ng)::value, kMaxT, kMinB>, p, s, (unsigned)grid);
+      if (p.part != nullptr) {
+        residual_norm_finish<<<dim3((p.d + 31) / 32, p.want_dpre + p.want_q), kFinishWarps * 32, 0, cur_stream()>>>(
+            p.part, (int)grid, p.d, p.want_dpre, p.alpha, a.gate_kind == kGateChannel ? p.gate : nullptr, p.post,
+            p.want_dpre ? dpre.data_ptr<float>() : nullptr, dpost.defined() ? dpost.data_ptr<float>() : nullptr,
+            gate_sum ? dgate.data_ptr<float>() : nullptr);
         MT_LAUNCH_CHECK();
       }
     });

@@ -56,6 +56,30 @@ __device__ __forceinline__ void store_stream(V* p, const V& a) {
   }
 }
 
+// Packed fp32 pairs: one instruction for two values (sm_100 f32x2), each rounded as on its own.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
+// 16-byte asynchronous copy global -> shared; nothing is read and zeros are written where `there` is false.
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool there) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most `pending` (0 .. 3) of this thread's youngest groups are in flight.
+__device__ __forceinline__ void copy_async_wait(int pending) {
+  if (pending >= 3)
+    asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (pending == 2)
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (pending == 1)
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 // f(T{}) with the activation type of a checked tensor.
 template <typename F>
 inline void dispatch_act(at::ScalarType t, F&& f) {
