@@ -47,6 +47,12 @@ at::Tensor rows_of(const at::Tensor& t) {
   return last_dense(r);
 }
 
+// The same for the norm kernels, whose rows are less than 2^31 values apart.
+at::Tensor near_rows_of(const at::Tensor& t) {
+  const at::Tensor r = rows_of(t);
+  return r.size(0) > 1 && r.stride(0) >= (int64_t(1) << 31) ? r.contiguous() : r;
+}
+
 at::Tensor or_undefined(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
@@ -267,11 +273,11 @@ int gate_kind(const at::Tensor& gate, const at::Tensor& x) {
 ResidualNormArgs norm_args(const at::Tensor& x, const at::Tensor& h, const at::Tensor& pre, const at::Tensor& post,
                            const at::Tensor& gate, int kind, double beta, double alpha, double eps) {
   ResidualNormArgs a;
-  a.x = rows_of(x);
-  if (h.defined()) a.h = rows_of(h);
+  a.x = near_rows_of(x);
+  if (h.defined()) a.h = near_rows_of(h);
   if (pre.defined()) a.pre = pre.contiguous();
   if (post.defined()) a.post = post.contiguous();
-  if (gate.defined()) a.gate = kind == kGateFull ? rows_of(gate) : gate.contiguous();
+  if (gate.defined()) a.gate = kind == kGateFull ? near_rows_of(gate) : gate.contiguous();
   a.gate_kind = kind;
   a.beta = beta;
   a.alpha = alpha;
@@ -336,7 +342,7 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
     at::Tensor dy = h.defined() ? g[at++] : at::Tensor(), dn = pre.defined() ? g[at] : at::Tensor();
     variable_list out(9);
     if (!dy.defined() && !dn.defined()) return out;
-    auto rows = [](const at::Tensor& t) { return t.defined() ? rows_of(t) : t; };
+    auto rows = [](const at::Tensor& t) { return t.defined() ? near_rows_of(t) : t; };
     // the node has an edge for each tensor that was given: i-th argument, next edge
     size_t edge = 0;
     for (size_t i = 0; i < 5; ++i) {

@@ -30,11 +30,12 @@ enum In : int { kX = 0, kH = 1, kGate = 2, kDy = 3, kDn = 4, kIns = 5 };
 
 struct NormParams {
   const void* in[kIns];  // nullptr: not there
-  int64_t ld[kIns];
+  uint32_t ld[kIns];
+  int slot[kIns];  // where an input lies in a row's slots, bytes
   const float *pre, *post, *gate;  // gate: per channel or per row
   void *y, *n, *dx, *dh, *dgate;
   float *rstd_h, *rstd_y, *part;
-  int64_t rows;
+  uint32_t rows;
   int d, gate_kind, depth, stage;  // ring: rows in flight, bytes of one row's slots
   float beta, alpha, eps;
   bool want_dpre, want_q;
@@ -55,32 +56,36 @@ template <typename T, bool ALIGNED, int NG>
 struct Rows {
   static constexpr int VEC = 16 / sizeof(T), NV = 8 / VEC;
   const NormParams& p;
-  unsigned char* ring;
-  int lane, g0;
+  const unsigned char* mine;  // this thread's first vector in the ring
+  uint32_t address;           // the same as a shared-memory address
+  int lane, g0, pitch;        // pitch: from a thread's vector to its next
 
-  __device__ __forceinline__ Rows(const NormParams& p, unsigned char* ring)
-      : p(p), ring(ring), lane(threadIdx.x & 31), g0((threadIdx.x >> 5) * NG) {}
+  __device__ __forceinline__ Rows(const NormParams& p, const unsigned char* ring)
+      : p(p),
+        mine(ring + threadIdx.x * 16),
+        address(static_cast<uint32_t>(__cvta_generic_to_shared(mine))),
+        lane(threadIdx.x & 31),
+        g0((threadIdx.x >> 5) * NG),
+        pitch(blockDim.x * 16) {}
 
-  __device__ __forceinline__ unsigned char* slot(int stage, int input, int k) const {
-    int at = 0;  // inputs before this one
-#pragma unroll
-    for (int t = 0; t < kIns; ++t) at += t < input && p.in[t] != nullptr;
-    return ring + stage * p.stage + ((at * NG * NV + k) * blockDim.x + threadIdx.x) * 16;
+  __device__ __forceinline__ const T* row_of(int t, uint32_t row) const {
+    return static_cast<const T*>(p.in[t]) + (uint64_t)row * p.ld[t];
   }
 
-  __device__ __forceinline__ void ask(int64_t row, int stage) const {
+  __device__ __forceinline__ void ask(uint32_t row, int stage) const {
     if constexpr (ALIGNED) {
       if (row < p.rows) {
 #pragma unroll
         for (int t = 0; t < kIns; ++t) {
           if (p.in[t] == nullptr) continue;
-          const T* src = static_cast<const T*>(p.in[t]) + row * p.ld[t];
+          const T* src = row_of(t, row);
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
               const int c = col_of<T, true>(g0 + g, lane, k * VEC);
-              copy_async16(slot(stage, t, g * NV + k), src + (c < p.d ? c : 0), c < p.d);
+              copy_async16(address + stage * p.stage + p.slot[t] + (g * NV + k) * pitch, src + (c < p.d ? c : 0),
+                           c < p.d);
             }
         }
       }
@@ -89,46 +94,58 @@ struct Rows {
   }
 
   // the 8 values of group g as pairs; 0 beyond d and where the input is not there
-  __device__ __forceinline__ void get(int input, int64_t row, int stage, int g, float2 (&f)[4]) const {
-    float v[8];
+  __device__ __forceinline__ void get(int input, uint32_t row, int stage, int g, float2 (&f)[4]) const {
     if (p.in[input] == nullptr) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      for (int i = 0; i < 4; ++i) f[i] = both(0.f);
     } else if constexpr (ALIGNED) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
-        widen(*reinterpret_cast<const Vec<T, VEC>*>(slot(stage, input, g * NV + k)), v + k * VEC);
+      for (int k = 0; k < NV; ++k) {
+        const uint4 w = *reinterpret_cast<const uint4*>(mine + stage * p.stage + p.slot[input] + (g * NV + k) * pitch);
+        if constexpr (sizeof(T) == 2) {
+          f[0] = widen_pair<T>(w.x);
+          f[1] = widen_pair<T>(w.y);
+          f[2] = widen_pair<T>(w.z);
+          f[3] = widen_pair<T>(w.w);
+        } else {
+          f[2 * k] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+          f[2 * k + 1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+        }
+      }
     } else {
-      const T* src = static_cast<const T*>(p.in[input]) + row * p.ld[input];
+      const T* src = row_of(input, row);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = col_of<T, false>(g0 + g, lane, i);
-        v[i] = c < p.d ? to_f<T>(src[c]) : 0.f;
+        const float v = c < p.d ? to_f<T>(src[c]) : 0.f;
+        if (i & 1)
+          f[i / 2].y = v;
+        else
+          f[i / 2].x = v;
       }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
   }
 
-  __device__ __forceinline__ void put(void* out, int64_t row, int g, const float2 (&f)[4]) const {
-    T* dst = static_cast<T*>(out) + row * p.d;
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = f[i].x;
-      v[2 * i + 1] = f[i].y;
-    }
+  __device__ __forceinline__ void put(void* out, uint32_t row, int g, const float2 (&f)[4]) const {
+    T* dst = static_cast<T*>(out) + (uint64_t)row * (uint32_t)p.d;
     if constexpr (ALIGNED) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = col_of<T, true>(g0 + g, lane, k * VEC);
-        if (c < p.d) store_stream(reinterpret_cast<Vec<T, VEC>*>(dst + c), narrow<T, VEC>(v + k * VEC));
+        uint4 w;
+        if constexpr (sizeof(T) == 2) {
+          w = make_uint4(narrow_pair<T>(f[0]), narrow_pair<T>(f[1]), narrow_pair<T>(f[2]), narrow_pair<T>(f[3]));
+        } else {
+          w = make_uint4(__float_as_uint(f[2 * k].x), __float_as_uint(f[2 * k].y), __float_as_uint(f[2 * k + 1].x),
+                         __float_as_uint(f[2 * k + 1].y));
+        }
+        if (c < p.d) __stcs(reinterpret_cast<uint4*>(dst + c), w);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = col_of<T, false>(g0 + g, lane, i);
-        if (c < p.d) dst[c] = from_f<T>(v[i]);
+        if (c < p.d) dst[c] = from_f<T>(i & 1 ? f[i / 2].y : f[i / 2].x);
       }
     }
   }
@@ -157,46 +174,42 @@ struct Rows {
 // halves, so that one barrier per call is enough.
 __device__ __forceinline__ float cta_sum(float v, float* red, int& par) {
   v = warp_sum(v);
-  const int nw = blockDim.x >> 5;
+  const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
   if (nw == 1) return v;
   float* r = red + par * kMaxWarps;
   par ^= 1;
-  if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+  if (lane == 0) r[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < nw; ++w) v += r[w];
-  return v;
+  return warp_sum(lane < nw ? r[lane] : 0.f);
 }
 
-// The same for four values: the halves of the warp first share the values out among them, so that 6 shuffles do.
+// The same for four values. The halves of the warp first share the values out among them, so that 6 shuffles do;
+// then a lane adds one value of every 8th warp.
 __device__ __forceinline__ float4 cta_sum4(float4 v, float4* red, int& par) {
+  constexpr unsigned kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const bool up = lane & 16, odd = lane & 8;
-  const float a = (up ? v.z : v.x) + __shfl_xor_sync(0xffffffffu, up ? v.x : v.z, 16);
-  const float b = (up ? v.w : v.y) + __shfl_xor_sync(0xffffffffu, up ? v.y : v.w, 16);
-  float s = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+  const float a = (up ? v.z : v.x) + __shfl_xor_sync(kAll, up ? v.x : v.z, 16);
+  const float b = (up ? v.w : v.y) + __shfl_xor_sync(kAll, up ? v.y : v.w, 16);
+  float s = (odd ? b : a) + __shfl_xor_sync(kAll, odd ? a : b, 8);
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
   // lanes 0, 8, 16, 24 hold the sums of x, y, z, w
   const int nw = blockDim.x >> 5;
-  if (nw == 1) {
-    v.x = __shfl_sync(0xffffffffu, s, 0);
-    v.y = __shfl_sync(0xffffffffu, s, 8);
-    v.z = __shfl_sync(0xffffffffu, s, 16);
-    v.w = __shfl_sync(0xffffffffu, s, 24);
-    return v;
+  int step = 8;
+  if (nw > 1) {
+    float* r = reinterpret_cast<float*>(red + par * kMaxWarps);
+    par ^= 1;
+    if ((lane & 7) == 0) r[(threadIdx.x >> 5) * 4 + (lane >> 3)] = s;
+    __syncthreads();
+    s = 0.f;
+    for (int i = lane; i < 4 * nw; i += 32) s += r[i];
+#pragma unroll
+    for (int o = 16; o > 2; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+    step = 1;  // lanes 0 .. 3
   }
-  float4* r = red + par * kMaxWarps;
-  par ^= 1;
-  if ((lane & 7) == 0) reinterpret_cast<float*>(r + (threadIdx.x >> 5))[lane >> 3] = s;
-  __syncthreads();
-  float2 lo = both(0.f), hi = both(0.f);
-  for (int w = 0; w < nw; ++w) {
-    const float4 t = r[w];
-    lo = add2(lo, make_float2(t.x, t.y));
-    hi = add2(hi, make_float2(t.z, t.w));
-  }
-  return make_float4(lo.x, lo.y, hi.x, hi.y);
+  return make_float4(__shfl_sync(kAll, s, 0), __shfl_sync(kAll, s, step), __shfl_sync(kAll, s, 2 * step),
+                     __shfl_sync(kAll, s, 3 * step));
 }
 
 template <typename T, bool ALIGNED, int NG, int MAXT, int MINB>
@@ -213,9 +226,9 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
     in.branch_weight(g, e[g]);
     in.weight(p.pre, g, 0.f, pre[g]);
   }
-  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + (int64_t)k * gridDim.x, k);
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    in.ask(row + (int64_t)(p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
+  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + k * gridDim.x, k);
+  for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    in.ask(row + (p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
     const float gate = p.gate_kind == kGateRow ? p.gate[row] : 1.f;
     if constexpr (ALIGNED) copy_async_wait(p.depth - 1);
     float2 y[NG][4];
@@ -291,16 +304,16 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
     for (int i = 0; i < 4; ++i) sum_pre[g][i] = sum_q[g][i] = both(0.f);
   }
   float next_rh = 1.f, next_ry = 0.f, next_gate = 1.f;
-  auto ask_scalars = [&](int64_t row) {
+  auto ask_scalars = [&](uint32_t row) {
     if (row >= p.rows) return;
     if (post) next_rh = p.rstd_h[row];
     if (p.in[kDn] != nullptr) next_ry = p.rstd_y[row];
     if (p.gate_kind == kGateRow) next_gate = p.gate[row];
   };
   ask_scalars(blockIdx.x);
-  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + (int64_t)k * gridDim.x, k);
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    in.ask(row + (int64_t)(p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
+  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + k * gridDim.x, k);
+  for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    in.ask(row + (p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
     const float rh = next_rh, ry = next_ry, gate = next_gate;
     ask_scalars(row + gridDim.x);
     if constexpr (ALIGNED) copy_async_wait(p.depth - 1);
@@ -460,6 +473,10 @@ void with_shape(const Shape& s, F&& f) {
 int64_t plan_ring(NormParams& p, const Shape& s, int esize, int fit, int deepest) {
   p.depth = 1;
   if (s.aligned) {
+    for (int t = 0, at = 0; t < kIns; ++t) {
+      p.slot[t] = at;
+      at += p.in[t] != nullptr ? s.groups * s.threads * 8 * esize : 0;
+    }
     p.stage = s.ins * s.groups * s.threads * 8 * esize;
     p.depth = std::min(deepest, std::max(1, kSmemBudget / fit / p.stage));
     fit = std::max(1, std::min(fit, kSmemBudget / (p.stage * p.depth)));
@@ -478,12 +495,14 @@ void launch_norm(K kernel, const NormParams& p, const Shape& s, unsigned grid) {
 
 const void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+uint32_t ld(const at::Tensor& t) { return t.defined() && t.size(0) > 1 ? (uint32_t)t.stride(0) : 0u; }
+
 NormParams params_of(const ResidualNormArgs& a) {
   NormParams p{};
   p.in[kX] = a.x.data_ptr();
-  p.rows = a.x.size(0);
+  MT_CHECK(a.x.size(0) < (int64_t(1) << 31), "residual_norm: too many rows: ", a.x.size(0));
+  p.rows = (uint32_t)a.x.size(0);
   p.d = (int)a.x.size(1);
-  auto ld = [](const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : int64_t(0); };
   p.ld[kX] = ld(a.x);
   if (a.h.has_value()) {
     p.in[kH] = a.h->data_ptr();
@@ -530,7 +549,6 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
                               const at::Tensor& dy, const at::Tensor& dn, const at::Tensor& dx, const at::Tensor& dh,
                               const at::Tensor& dgate, const at::Tensor& dpre, const at::Tensor& dpost) {
   NormParams p = params_of(a);
-  auto ld = [](const at::Tensor& t) { return t.defined() && t.size(0) > 1 ? t.stride(0) : int64_t(0); };
   p.in[kDy] = ptr(dy);
   p.ld[kDy] = ld(dy);
   p.in[kDn] = ptr(dn);
@@ -560,7 +578,7 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
       at::Tensor part;
       if (p.want_dpre || p.want_q) {
         // a few rows for each CTA at least: its partial sums cost as much as two rows
-        grid = std::min(grid, (p.rows + 3) / 4);
+        grid = std::min<int64_t>(grid, (p.rows + 3) / 4);
         part = at::empty({grid, 2, (int64_t)p.d}, a.x.options().dtype(at::kFloat));
         p.part = part.data_ptr<float>();
       }

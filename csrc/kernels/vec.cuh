@@ -10,18 +10,58 @@ struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
 
+// A pair of 16-bit values in one 32-bit word, lower half first.
+template <typename T>
+__device__ __forceinline__ float2 widen_pair(uint32_t w);
+template <>
+__device__ __forceinline__ float2 widen_pair<bf16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 widen_pair<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow_pair(float2 f);
+template <>
+__device__ __forceinline__ uint32_t narrow_pair<bf16>(float2 f) {
+  const bf162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t narrow_pair<__half>(float2 f) {
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void widen(const Vec<T, N>& a, float* f) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&a);
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = to_f<T>(a.v[i]);
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 t = widen_pair<T>(w[i]);
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f<T>(a.v[i]);
+  }
 }
 
 // One rounding to nearest of each value.
 template <typename T, int N>
 __device__ __forceinline__ Vec<T, N> narrow(const float* f) {
   Vec<T, N> a;
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&a);
 #pragma unroll
-  for (int i = 0; i < N; ++i) a.v[i] = from_f<T>(f[i]);
+    for (int i = 0; i < N / 2; ++i) w[i] = narrow_pair<T>(make_float2(f[2 * i], f[2 * i + 1]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.v[i] = from_f<T>(f[i]);
+  }
   return a;
 }
 
@@ -62,9 +102,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 
-// 16-byte asynchronous copy global -> shared; nothing is read and zeros are written where `there` is false.
-__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool there) {
-  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+// 16-byte asynchronous copy global -> shared (address d); nothing is read and zeros are written where `there` is false.
+__device__ __forceinline__ void copy_async16(uint32_t d, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
