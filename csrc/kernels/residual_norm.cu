@@ -51,8 +51,9 @@ __device__ __forceinline__ int col_of(int group, int lane, int i) {
 }
 
 // The rows that a thread has asked for, and their values. The slots of one row lie one input after another, each
-// with one 16-byte vector of every thread after the other.
-template <typename T, bool ALIGNED, int NG>
+// with one 16-byte vector of every thread after the other. INPUTS: a bit for each input, or 0 where the kernel looks
+// at its parameters for which ones there are.
+template <typename T, bool ALIGNED, int NG, unsigned INPUTS>
 struct Rows {
   static constexpr int VEC = 16 / sizeof(T), NV = 8 / VEC;
   const NormParams& p;
@@ -68,6 +69,8 @@ struct Rows {
         g0((threadIdx.x >> 5) * NG),
         pitch(blockDim.x * 16) {}
 
+  __device__ __forceinline__ bool has(int t) const { return INPUTS != 0 ? INPUTS >> t & 1 : p.in[t] != nullptr; }
+
   __device__ __forceinline__ const T* row_of(int t, uint32_t row) const {
     return static_cast<const T*>(p.in[t]) + (uint64_t)row * p.ld[t];
   }
@@ -77,7 +80,7 @@ struct Rows {
       if (row < p.rows) {
 #pragma unroll
         for (int t = 0; t < kIns; ++t) {
-          if (p.in[t] == nullptr) continue;
+          if (!has(t)) continue;
           const T* src = row_of(t, row);
 #pragma unroll
           for (int g = 0; g < NG; ++g)
@@ -95,7 +98,7 @@ struct Rows {
 
   // the 8 values of group g as pairs; 0 beyond d and where the input is not there
   __device__ __forceinline__ void get(int input, uint32_t row, int stage, int g, float2 (&f)[4]) const {
-    if (p.in[input] == nullptr) {
+    if (!has(input)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = both(0.f);
     } else if constexpr (ALIGNED) {
@@ -212,13 +215,15 @@ __device__ __forceinline__ float4 cta_sum4(float4 v, float4* red, int& par) {
                      __shfl_sync(kAll, s, 3 * step));
 }
 
-template <typename T, bool ALIGNED, int NG, int MAXT, int MINB>
+// ALL: there are a branch and a pre norm, and no gate per element -- what a training step calls; with this known, and
+// the rest done by arithmetic (no post norm is rh = 1), a row takes two thirds of the instructions.
+template <typename T, bool ALIGNED, int NG, bool ALL, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[2 * kMaxWarps];
-  const Rows<T, ALIGNED, NG> in(p, ring);
+  const Rows<T, ALIGNED, NG, ALL ? 1u << kX | 1u << kH : 0u> in(p, ring);
   const float inv_d = 1.f / p.d;
-  const bool branch = p.in[kH] != nullptr;
+  const bool branch = in.has(kH);
   int par = 0, stage = 0;
   float2 e[NG][4], pre[NG][4];
 #pragma unroll
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
         in.get(kX, row, stage, g, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[g][i] = mul2(y[g][i], e[g][i]);
-        if (p.gate_kind == kGateFull) {
+        if (!ALL && p.gate_kind == kGateFull) {
           float2 w[4];
           in.get(kGate, row, stage, g, w);
 #pragma unroll
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
 #pragma unroll
       for (int g = 0; g < NG; ++g) in.get(kX, row, stage, g, y[g]);
     }
-    if (p.n != nullptr) {
+    if (ALL || p.n != nullptr) {
       float2 s = both(0.f);
 #pragma unroll
       for (int g = 0; g < NG; ++g)
@@ -287,19 +292,20 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
 }
 
 // part: [gridDim.x][2][d], the CTA's sums of dn yh (dpre) and of r Y hh (q; with the gate of each element)
-template <typename T, bool ALIGNED, int NG, int MAXT, int MINB>
+// ALL: as in the forward, and both gradients come in and both are wanted.
+template <typename T, bool ALIGNED, int NG, bool ALL, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float4 red[2 * kMaxWarps];
-  const Rows<T, ALIGNED, NG> in(p, ring);
+  const Rows<T, ALIGNED, NG, ALL ? 1u << kX | 1u << kH | 1u << kDy | 1u << kDn : 0u> in(p, ring);
   const float inv_d = 1.f / p.d;
-  const bool branch = p.in[kH] != nullptr, full = p.gate_kind == kGateFull, post = p.post != nullptr;
+  const bool branch = in.has(kH), full = !ALL && p.gate_kind == kGateFull, post = p.post != nullptr;
   int par = 0, stage = 0;
   float2 e[NG][4], pre[NG][4], sum_pre[NG][4], sum_q[NG][4];
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     in.branch_weight(g, e[g]);
-    in.weight(p.in[kDn] != nullptr ? p.pre : nullptr, g, 0.f, pre[g]);
+    in.weight(in.has(kDn) ? p.pre : nullptr, g, 0.f, pre[g]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum_pre[g][i] = sum_q[g][i] = both(0.f);
   }
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
   auto ask_scalars = [&](uint32_t row) {
     if (row >= p.rows) return;
     if (post) next_rh = p.rstd_h[row];
-    if (p.in[kDn] != nullptr) next_ry = p.rstd_y[row];
+    if (in.has(kDn)) next_ry = p.rstd_y[row];
     if (p.gate_kind == kGateRow) next_gate = p.gate[row];
   };
   ask_scalars(blockIdx.x);
@@ -353,7 +359,8 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
     const float m = s.x * inv_d;
     const float cy = s.y + ry * (s.z - m * s.w);  // sum of c Y
     if (p.gate_kind == kGateRow && p.dgate != nullptr && threadIdx.x == 0) static_cast<float*>(p.dgate)[row] = cy;
-    const float2 minus_m = both(-m), minus_k = both(-rh * gate * cy * inv_d), r = both(post ? rh * gate : gate);
+    // without a post norm rh is 1 and dh has no mean
+    const float2 minus_m = both(-m), minus_k = both(post ? -rh * gate * cy * inv_d : 0.f), r = both(rh * gate);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float2 o[4];
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
         dy[g][i] = fma2(fma2(yh[g][i], minus_m, u[g][i]), both(ry), dy[g][i]);  // Y
         o[i] = mul2(dy[g][i], both(p.beta));
       }
-      if (p.dx != nullptr) in.put(p.dx, row, g, o);
+      if (ALL || p.dx != nullptr) in.put(p.dx, row, g, o);
       if (!branch) continue;
       if (full) {
         float2 w[4];
@@ -378,10 +385,9 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         sum_q[g][i] = fma2(mul2(dy[g][i], both(gate)), hh[g][i], sum_q[g][i]);
-        o[i] = mul2(mul2(dy[g][i], e[g][i]), r);
-        if (post) o[i] = fma2(hh[g][i], minus_k, o[i]);
+        o[i] = fma2(hh[g][i], minus_k, mul2(mul2(dy[g][i], e[g][i]), r));
       }
-      if (p.dh != nullptr) in.put(p.dh, row, g, o);
+      if (ALL || p.dh != nullptr) in.put(p.dh, row, g, o);
     }
     stage = stage + 1 == p.depth ? 0 : stage + 1;
   }
@@ -449,24 +455,26 @@ Shape shape_of(const NormParams& p, int esize) {
   return Shape{ok, threads, groups, ins};
 }
 
-// f(ALIGNED, NG, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
+// f(ALIGNED, NG, ALL, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
 template <typename F>
-void with_shape(const Shape& s, F&& f) {
-  auto go = [&](auto al) {
-    using std::integral_constant;
+void with_shape(const Shape& s, bool all, F&& f) {
+  using std::integral_constant;
+  auto go = [&](auto al, auto every) {
     if (s.groups == 2)
-      f(al, integral_constant<int, 2>{}, integral_constant<int, 1024>{});
+      f(al, integral_constant<int, 2>{}, every, integral_constant<int, 1024>{});
     else if (s.threads > 512)
-      f(al, integral_constant<int, 1>{}, integral_constant<int, 1024>{});
+      f(al, integral_constant<int, 1>{}, every, integral_constant<int, 1024>{});
     else if (s.threads > 256)
-      f(al, integral_constant<int, 1>{}, integral_constant<int, 512>{});
+      f(al, integral_constant<int, 1>{}, every, integral_constant<int, 512>{});
     else
-      f(al, integral_constant<int, 1>{}, integral_constant<int, 256>{});
+      f(al, integral_constant<int, 1>{}, every, integral_constant<int, 256>{});
   };
-  if (s.aligned)
-    go(std::true_type{});
+  if (s.aligned && all)
+    go(std::true_type{}, std::true_type{});
+  else if (s.aligned)
+    go(std::true_type{}, std::false_type{});
   else
-    go(std::false_type{});
+    go(std::false_type{}, std::false_type{});
 }
 
 // The ring's depth for `fit` CTAs per SM, and the CTAs that are resident with it.
@@ -536,11 +544,12 @@ void residual_norm_fwd_launch(const ResidualNormArgs& a, const at::Tensor& y, co
   dispatch_act(a.x.scalar_type(), [&](auto t) {
     using T = decltype(t);
     const Shape s = shape_of(p, sizeof(T));
-    with_shape(s, [&](auto al, auto ng, auto maxt) {
+    const bool all = p.in[kH] != nullptr && p.n != nullptr && a.gate_kind != kGateFull;
+    with_shape(s, all, [&](auto al, auto ng, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 1024 ? 1 : 1024 / kMaxT;
       const int fit = std::min(16, kMinB * kMaxT / s.threads);
       const unsigned grid = (unsigned)std::min<int64_t>(p.rows, plan_ring(p, s, sizeof(T), fit, 4));
-      launch_norm(residual_norm_fwd<T, decltype(al)::value, decltype(ng)::value, kMaxT, kMinB>, p, s, grid);
+      launch_norm(residual_norm_fwd<T, decltype(al)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, grid);
     });
   });
 }
@@ -571,7 +580,9 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
   dispatch_act(a.x.scalar_type(), [&](auto t) {
     using T = decltype(t);
     const Shape s = shape_of(p, sizeof(T));
-    with_shape(s, [&](auto al, auto ng, auto maxt) {
+    bool all = a.gate_kind != kGateFull;
+    for (const void* q : {p.in[kH], p.in[kDy], p.in[kDn], (const void*)p.dx, (const void*)p.dh}) all = all && q != nullptr;
+    with_shape(s, all, [&](auto al, auto ng, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 256 ? 2 : 1;
       const int fit = std::min(16, kMinB * kMaxT / s.threads);
       int64_t grid = std::min<int64_t>(p.rows, plan_ring(p, s, sizeof(T), fit, 4));
@@ -582,7 +593,7 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
         part = at::empty({grid, 2, (int64_t)p.d}, a.x.options().dtype(at::kFloat));
         p.part = part.data_ptr<float>();
       }
-      launch_norm(residual_norm_bwd<T, decltype(al)::value, decltype(ng)::value, kMaxT, kMinB>, p, s, (unsigned)grid);
+      launch_norm(residual_norm_bwd<T, decltype(al)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, (unsigned)grid);
       if (p.part != nullptr) {
         residual_norm_finish<<<dim3((p.d + 31) / 32, p.want_dpre + p.want_q), kFinishWarps * 32, 0, cur_stream()>>>(
             p.part, (int)grid, p.d, p.want_dpre, p.alpha, a.gate_kind == kGateChannel ? p.gate : nullptr, p.post,
