@@ -2,6 +2,7 @@
 // gradients.  The autograd nodes are C++ because the smallest calls (one decoding step) are bound by the time to
 // get from Python to the launch.
 #include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -36,6 +37,12 @@ void check_cuda(std::initializer_list<const at::Tensor*> ts, const char* op) {
                 " and ", t->device(), ")");
   }
 }
+
+// Uninitialised memory on t's device, without the way through the dispatcher.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& t) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, t.device(), c10::nullopt));
+}
+at::Tensor fresh_like(const at::Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
 
 at::Tensor last_dense(const at::Tensor& t) {
   return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
@@ -125,7 +132,7 @@ std::vector<at::Tensor> rotary_raw(const std::vector<at::Tensor>& xs, const Rota
   std::vector<at::Tensor> outs;
   for (size_t i = 0; i < xs.size(); ++i) {
     const at::Tensor in = last_dense(xs[i]);
-    outs.push_back(at::empty(xs[i].sizes(), xs[i].options()));
+    outs.push_back(fresh_like(xs[i]));
     segs.push_back({tokens_of(in), tokens_of(outs[i]), heads_rot[i]});
   }
   rotary_launch(segs, RotaryArgs{r.turns, r.rot_dim, r.interleaved, r.scale, positions, offset, inverse});
@@ -300,10 +307,10 @@ NormOutputs norm_forward(const at::Tensor& x, const at::Tensor& h, const at::Ten
   c10::cuda::CUDAGuard guard(x.device());
   const ResidualNormArgs a = norm_args(x, h, pre, post, gate, kind, beta, alpha, eps);
   NormOutputs o;
-  if (h.defined()) o.y = at::empty(x.sizes(), x.options());
-  if (pre.defined()) o.n = at::empty(x.sizes(), x.options());
+  if (h.defined()) o.y = fresh_like(x);
+  if (pre.defined()) o.n = fresh_like(x);
   if (statistics) {
-    const at::Tensor stats = at::empty({2, a.x.size(0)}, x.options().dtype(at::kFloat));
+    const at::Tensor stats = fresh({2, a.x.size(0)}, at::kFloat, x);
     if (post.defined()) o.rstd_h = stats.select(0, 0);
     if (pre.defined()) o.rstd_y = stats.select(0, 1);
   }
@@ -347,7 +354,7 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
     size_t edge = 0;
     for (size_t i = 0; i < 5; ++i) {
       if (s[i].defined() && ctx->needs_input_grad(edge++) && !(i == 2 && !dn.defined()))
-        out[i] = at::empty(s[i].sizes(), s[i].options());
+        out[i] = fresh_like(s[i]);
     }
     residual_norm_bwd_launch(a, s[5], s[6], rows(dy), rows(dn), out[0], out[1], out[4], out[2], out[3]);
     return out;
@@ -420,17 +427,16 @@ LogprobOutputs logprobs_forward(const at::Tensor& logits, const at::Tensor& toke
                                 bool entropy) {
   c10::cuda::CUDAGuard guard(logits.device());
   const at::Tensor x = rows_of(logits);
-  const auto f32 = logits.options().dtype(at::kFloat);
   LogprobOutputs o;
   o.tokens = tokens.dim() == 1 ? tokens.contiguous() : tokens.reshape({-1}).contiguous();
-  o.logprob = at::empty(tokens.sizes(), f32);
-  o.stats = at::empty({x.size(0), 2}, f32);
-  if (entropy) o.entropy = at::empty(tokens.sizes(), f32);
+  o.logprob = fresh(tokens.sizes(), at::kFloat, logits);
+  o.stats = fresh({x.size(0), 2}, at::kFloat, logits);
+  if (entropy) o.entropy = fresh(tokens.sizes(), at::kFloat, logits);
   if (top > 0) {
     std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
     shape.push_back(top);
-    o.top_lp = at::empty(shape, f32);
-    o.top_ids = at::empty(shape, tokens.options());
+    o.top_lp = fresh(shape, at::kFloat, logits);
+    o.top_ids = fresh(shape, at::kLong, logits);
   }
   token_logprobs_fwd_launch(x, o.tokens, inv_tau, top, o.logprob, o.stats, o.entropy, o.top_lp, o.top_ids);
   return o;
@@ -464,7 +470,7 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
     const at::Tensor gl = next(true), gh = next(entropy), gk = next(top > 0);
     variable_list out(5);
     if (!gl.defined() && !gh.defined() && !gk.defined()) return out;
-    out[0] = at::empty(s[0].sizes(), s[0].options());
+    out[0] = fresh_like(s[0]);
     token_logprobs_bwd_launch(rows_of(s[0]), s[1], ctx->saved_data["inv_tau"].toDouble(), top, s[2], s[3], s[4], gl,
                               gh, gk, out[0]);
     return out;

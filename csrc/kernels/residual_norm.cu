@@ -15,6 +15,8 @@
 // The backward needs little more than the memory's time in instructions, so it is written to need few: one row
 // reduction, not two (mean(e hh Y) follows from sums of e hh with dy + ry u and with yh), one column sum q = sum r Y hh for
 // both dpost = alpha g q and dgate = alpha post q, pairs of values per instruction, and 6 shuffles for 3 row sums.
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "decoder_ops.h"
 #include "vec.cuh"
 
@@ -603,7 +605,7 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
       if (p.want_dpre || p.want_q) {
         // a few rows for each CTA at least: its partial sums cost as much as two rows
         grid = std::min<int64_t>(grid, (p.rows + 3) / 4);
-        part = at::empty({grid, 2, (int64_t)p.d}, a.x.options().dtype(at::kFloat));
+        part = at::Tensor(at::detail::empty_cuda({grid, 2, (int64_t)p.d}, at::kFloat, a.x.device(), c10::nullopt));
         p.part = part.data_ptr<float>();
       }
       launch_norm(residual_norm_bwd<T, decltype(al)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, (unsigned)grid);

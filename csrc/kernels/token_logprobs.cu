@@ -79,13 +79,116 @@ __device__ __forceinline__ void join(Running& a, Running b, float c) {
   a.w += b.w;
 }
 
+// One value, whatever it is: NaN and inf - inf go on into the sums, a masked value adds 2^-200 * -200 = 0.
 template <bool ENT>
 __device__ __forceinline__ void add(Running& a, float x, float c) {
-  // NaN and inf - inf go on into the sums; a masked value adds 2^-200 * -200 = 0
+  if (x > a.m) rescale(a, x, c);
   const float t = ENT ? max_nan((x - a.m) * c, -200.f) : (x - a.m) * c;
   const float e = ex2(t);
   a.s += e;
   if (ENT) a.w = fmaf(e, t, a.w);
+}
+
+// Packed maximum of two 16-bit values each: a NaN loses, or wins.
+template <typename T>
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  uint32_t y;
+  if constexpr (std::is_same_v<T, bf16>)
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  else
+    asm("max.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max_pair_nan(uint32_t a, uint32_t b) {
+  uint32_t y;
+  if constexpr (std::is_same_v<T, bf16>)
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ float largest(const Vec<T, 16 / sizeof(T)>& v) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+    const float2 f = widen_pair<T>(max_pair<T>(max_pair<T>(w[0], w[1]), max_pair<T>(w[2], w[3])));
+    return fmaxf(f.x, f.y);
+  } else {
+    return fmaxf(fmaxf(v.v[0], v.v[1]), fmaxf(v.v[2], v.v[3]));
+  }
+}
+
+// A thread's sums over its vectors with few instructions per value: exponents x c - r with the reference r = m c,
+// two values at a time. r is rounded; that shifts all exponents alike and fast_done() takes it out again. For the
+// weighted sum, values are kept at -1e30 or above (fp16: at its lowest), so that an exponent is finite and a masked
+// value adds 0 * finite. Good for maxima from -2^26 / c to 2^26 / c that lie well above that; fast_done() says so.
+struct Fast {
+  float m, r, best;  // m >= the lower limit; best: the largest value
+  float2 s, w;
+};
+
+constexpr float kFastLimit = 67108864.f;  // 2^26: r is rounded by at most 2
+
+__device__ __forceinline__ Fast fast_start(float c) {
+  return Fast{-kFastLimit / c, -kFastLimit, -INFINITY, both(0.f), both(0.f)};
+}
+
+// A vector with a value above `best`.
+template <bool ENT>
+__device__ __forceinline__ void fast_raise(Fast& a, float vm, float c) {
+  a.best = vm;
+  if (vm <= a.m) return;
+  const float r = vm * c, d = a.r - r, f = ex2(d);
+  if (ENT) a.w = mul2(fma2(a.s, both(d), a.w), both(f));
+  a.s = mul2(a.s, both(f));
+  a.m = vm;
+  a.r = r;
+}
+
+template <typename T>
+__device__ __forceinline__ constexpr float kept_above() {
+  return std::is_same_v<T, __half> ? -65504.f : -1e30f;
+}
+
+template <typename T, bool ENT>
+__device__ __forceinline__ void fast_add(Fast& a, const Vec<T, 16 / sizeof(T)>& v, float c) {
+  constexpr int N = 16 / sizeof(T) / 2;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float2 x;
+    if constexpr (sizeof(T) == 2) {
+      uint32_t w = reinterpret_cast<const uint32_t*>(&v)[i];
+      if (ENT) w = max_pair_nan<T>(w, std::is_same_v<T, bf16> ? 0xf149f149u : 0xfbfffbffu);  // kept_above<T>()
+      x = widen_pair<T>(w);
+    } else {
+      x = make_float2(v.v[2 * i], v.v[2 * i + 1]);
+      if (ENT) x = make_float2(max_nan(x.x, kept_above<T>()), max_nan(x.y, kept_above<T>()));
+    }
+    const float2 t = fma2(x, both(c), both(-a.r));
+    const float2 e = make_float2(ex2(t.x), ex2(t.y));
+    a.s = add2(a.s, e);
+    if (ENT) a.w = fma2(e, t, a.w);
+  }
+}
+
+// The sums relative to the maximum itself; false where the values were out of range (a NaN or +inf among them shows
+// in the sums and needs no second look).
+template <typename T, bool ENT>
+__device__ __forceinline__ bool fast_done(const Fast& a, float c, Running& out) {
+  const float s = a.s.x + a.s.y, w = a.w.x + a.w.y;
+  out = Running{kLowest, 0.f, 0.f};
+  if (isnan(s)) {
+    out.s = s;
+    return true;
+  }
+  if (a.best == -INFINITY) return true;  // nothing, or masked values only
+  if (a.best < a.m || fabsf(a.r) > kFastLimit) return false;
+  if (ENT && (kept_above<T>() - a.m) * c > -200.f) return false;
+  const float d = fmaf(a.m, c, -a.r), f = ex2(-d);
+  out = Running{a.m, s * f, f * fmaf(-d, s, w)};
+  return true;
 }
 
 __device__ __forceinline__ Running shuffle_join(Running a, float c) {
@@ -162,22 +265,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_fwd(const __grid_cons
   const int64_t step = (int64_t)kThreads * C, first = (int64_t)rank * kThreads + tid;
 
   // one pass: vector j of the row belongs to thread j % (kThreads C) of the cluster
-  Running a{kLowest, 0.f, 0.f};
-  float best = -INFINITY;
+  Fast sums = fast_start(p.c);
   int64_t best_at = first;
   auto take = [&](const V16& v, int64_t j) {
-    float f[VEC];
-    widen(v, f);
-    float vm = f[0];
-#pragma unroll
-    for (int i = 1; i < VEC; ++i) vm = fmaxf(vm, f[i]);
-    if (TOP && vm > best) {
-      best = vm;
+    const float vm = largest<T>(v);
+    if (vm > sums.best) {
       best_at = j;
+      fast_raise<ENT>(sums, vm, p.c);
     }
-    if (vm > a.m) rescale(a, vm, p.c);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) add<ENT>(a, f[i], p.c);
+    fast_add<T, ENT>(sums, v, p.c);
   };
   int64_t j = first;
   for (; j + (UNROLL - 1) * step < parts.vectors; j += UNROLL * step) {
@@ -188,14 +284,19 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_fwd(const __grid_cons
     for (int u = 0; u < UNROLL; ++u) take(v[u], j + u * step);
   }
   for (; j < parts.vectors; j += step) take(xv[j], j);
+  Running a;
+  if (!fast_done<T, ENT>(sums, p.c, a)) {
+    for (j = first; j < parts.vectors; j += step) {
+      float f[VEC];
+      widen(xv[j], f);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) add<ENT>(a, f[i], p.c);
+    }
+  }
   // the row's ends: at most 2 (VEC - 1) values, one each for the first threads of the cluster
   const int64_t ends = parts.head + (p.V - parts.tail0);
   const int64_t end_at = first < parts.head ? first : parts.tail0 + (first - parts.head);
-  if (first < ends) {
-    const float f = to_f<T>(x[end_at]);
-    if (f > a.m) rescale(a, f, p.c);
-    add<ENT>(a, f, p.c);
-  }
+  if (first < ends) add<ENT>(a, to_f<T>(x[end_at]), p.c);
 
   a = shuffle_join(a, p.c);
   if ((tid & 31) == 0) warps[tid >> 5] = a;
