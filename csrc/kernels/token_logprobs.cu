@@ -10,11 +10,14 @@
 // memory and, across the cluster, distributed shared memory.  Exponentials are base 2 of differences to the running
 // maximum, subtracted before they are scaled, so that a row of the type's lowest values stays uniform.
 //
-// The alternatives cost no second pass: the maximum of each group of 4 threads is known after the first.  With k
-// groups' maxima at or above the k-th largest of them, every value of the top k lies in one of these groups, so only
-// their vectors are read again (from L2) and compared.  Values order by (value, lowest index) as one 64-bit key, so
-// there are no ties.
+// The alternatives take a second, small kernel.  The first leaves the maxima of small groups of neighbouring values.
+// The k-th largest of them bounds the k-th largest value from below, and only a group whose maximum reaches it can hold
+// one of the k: these few groups are read again and their values from the bound on are ranked.  Values order by
+// (value, lowest index) as one 64-bit key, so there are no ties.  In one kernel with the pass over the logits the same
+// steps were slower, since each of them waits for memory behind the loads of the other rows on its SM.
 #include <cooperative_groups.h>
+
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "decoder_ops.h"
 #include "vec.cuh"
@@ -25,10 +28,14 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kGroups = kThreads / 4;
+constexpr int kThreads = 256;  // of a CTA of the first pass and of the backward
+constexpr int kUnroll = 4;     // vectors of a thread in flight
+constexpr int kTile = kThreads * kUnroll;
+constexpr int kSelThreads = 128;
+constexpr int kColumns = 2 * kSelThreads;
+constexpr int kMaxWinners = 128;
 constexpr int kMaxTop = 64;
-constexpr int kCandidates = 1024;
+constexpr int kHits = 512, kCandidates = 768;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;  // finite, so that differences to it are never NaN
 constexpr long long kNoKey = LLONG_MIN;
@@ -47,11 +54,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
-// Orders by value, then by lowest index; -0 equals 0 and NaN ranks with -inf.
-__device__ __forceinline__ long long key_of(float x, int64_t index) {
+// Whole numbers in the order of the values; -0 equals 0 and NaN ranks with -inf.
+__device__ __forceinline__ int order_of(float x) {
   const int b = __float_as_int(isnan(x) ? -INFINITY : x);
-  const int o = b < 0 ? -(b & 0x7fffffff) : b;
-  return (long long)o * 0x100000000ll + (0xffffffffll - index);
+  return b < 0 ? -(b & 0x7fffffff) : b;
+}
+// Keys order by value, then by lowest index.
+__device__ __forceinline__ long long key_of(float x, int64_t index) {
+  return (long long)order_of(x) * 0x100000000ll + (0xffffffffll - index);
 }
 __device__ __forceinline__ float key_value(long long k) {
   const int o = (int)(k >> 32);
@@ -109,42 +119,49 @@ __device__ __forceinline__ uint32_t max_pair_nan(uint32_t a, uint32_t b) {
   return y;
 }
 
-template <typename T>
-__device__ __forceinline__ float largest(const Vec<T, 16 / sizeof(T)>& v) {
+// The largest value of N vectors.
+template <typename T, int N>
+__device__ __forceinline__ float largest(const Vec<T, 16 / sizeof(T)> (&v)[N]) {
   if constexpr (sizeof(T) == 2) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
-    const float2 f = widen_pair<T>(max_pair<T>(max_pair<T>(w[0], w[1]), max_pair<T>(w[2], w[3])));
+    uint32_t m = reinterpret_cast<const uint32_t*>(&v[0])[0];
+#pragma unroll
+    for (int i = 1; i < 4 * N; ++i) m = max_pair<T>(m, reinterpret_cast<const uint32_t*>(&v[i / 4])[i % 4]);
+    const float2 f = widen_pair<T>(m);
     return fmaxf(f.x, f.y);
   } else {
-    return fmaxf(fmaxf(v.v[0], v.v[1]), fmaxf(v.v[2], v.v[3]));
+    float m = v[0].v[0];
+#pragma unroll
+    for (int i = 1; i < 4 * N; ++i) m = fmaxf(m, v[i / 4].v[i % 4]);
+    return m;
   }
 }
 
 // A thread's sums over its vectors with few instructions per value: exponents x c - r with the reference r = m c,
-// two values at a time. r is rounded; that shifts all exponents alike and fast_done() takes it out again. For the
-// weighted sum, values are kept at -1e30 or above (fp16: at its lowest), so that an exponent is finite and a masked
-// value adds 0 * finite. Good for maxima from -2^26 / c to 2^26 / c that lie well above that; fast_done() says so.
+// two values at a time. m follows the maximum only when that is 2^8 times likelier, so that hardly any vector after
+// the first has to rescale the sums (a warp does when one of its lanes does). r is rounded; that shifts all exponents
+// alike and fast_done() takes it out again. For the weighted sum, values are kept at -1e30 or above (fp16: at its
+// lowest), so that an exponent is finite and a masked value adds 0 * finite. Good for maxima from -2^26 / c to
+// 2^26 / c that lie well above that; fast_done() says so.
 struct Fast {
-  float m, r, best;  // m >= the lower limit; best: the largest value
+  float m, minus_r, limit, best;  // limit: the maximum up to which m stays; best: the maximum
   float2 s, w;
 };
 
 constexpr float kFastLimit = 67108864.f;  // 2^26: r is rounded by at most 2
+constexpr float kSlack = 8.f;
 
 __device__ __forceinline__ Fast fast_start(float c) {
-  return Fast{-kFastLimit / c, -kFastLimit, -INFINITY, both(0.f), both(0.f)};
+  return Fast{-kFastLimit / c, kFastLimit, -kFastLimit / c, -INFINITY, both(0.f), both(0.f)};
 }
 
-// A vector with a value above `best`.
 template <bool ENT>
 __device__ __forceinline__ void fast_raise(Fast& a, float vm, float c) {
-  a.best = vm;
-  if (vm <= a.m) return;
-  const float r = vm * c, d = a.r - r, f = ex2(d);
+  const float minus_r = -(vm * c), d = minus_r - a.minus_r, f = ex2(d);
   if (ENT) a.w = mul2(fma2(a.s, both(d), a.w), both(f));
   a.s = mul2(a.s, both(f));
   a.m = vm;
-  a.r = r;
+  a.minus_r = minus_r;
+  a.limit = vm + kSlack / c;
 }
 
 template <typename T>
@@ -166,7 +183,7 @@ __device__ __forceinline__ void fast_add(Fast& a, const Vec<T, 16 / sizeof(T)>& 
       x = make_float2(v.v[2 * i], v.v[2 * i + 1]);
       if (ENT) x = make_float2(max_nan(x.x, kept_above<T>()), max_nan(x.y, kept_above<T>()));
     }
-    const float2 t = fma2(x, both(c), both(-a.r));
+    const float2 t = fma2(x, both(c), both(a.minus_r));
     const float2 e = make_float2(ex2(t.x), ex2(t.y));
     a.s = add2(a.s, e);
     if (ENT) a.w = fma2(e, t, a.w);
@@ -184,9 +201,9 @@ __device__ __forceinline__ bool fast_done(const Fast& a, float c, Running& out) 
     return true;
   }
   if (a.best == -INFINITY) return true;  // nothing, or masked values only
-  if (a.best < a.m || fabsf(a.r) > kFastLimit) return false;
+  if (a.best < a.m || fabsf(a.minus_r) > kFastLimit) return false;  // below the lower limit, or above the upper
   if (ENT && (kept_above<T>() - a.m) * c > -200.f) return false;
-  const float d = fmaf(a.m, c, -a.r), f = ex2(-d);
+  const float d = fmaf(a.m, c, a.minus_r), f = ex2(-d);
   out = Running{a.m, s * f, f * fmaf(-d, s, w)};
   return true;
 }
@@ -219,216 +236,332 @@ struct RowParts {
 struct FwdParams {
   const void* logits;
   const int64_t* tokens;
-  float *logprob, *stats, *entropy, *top_lp;
-  int64_t* top_ids;
-  int64_t ld, V;
+  float *logprob, *stats, *entropy;
+  float* maxima;  // [rows, tiles, kThreads >> lanes_log], or nullptr; -inf for a group without values
+  int64_t ld, V, tiles;  // tiles: of the row with the most
   float c, inv_tau;
-  int top, cluster;
+  int cluster, lanes_log;
 };
-
-struct TopShared {
-  long long group[kGroups];
-  long long cand[kCandidates];
-  long long best[kMaxTop];  // this CTA's largest keys in falling order, kNoKey behind them
-  int winners[kGroups];
-  int n_cand, n_winners;
-  long long threshold, red[kThreads / 32];
-};
-
-// Writes the `top` largest of keys[0, n) to out in falling order. The keys differ, but for kNoKey, which is left
-// out; with fewer than `top` keys, kNoKey follows them where n < top.
-__device__ __forceinline__ void rank_keys(const long long* keys, int n, long long* out, int top) {
-  for (int i = n + threadIdx.x; i < top; i += kThreads) out[i] = kNoKey;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const long long k = keys[i];
-    if (k == kNoKey) continue;
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += keys[j] > k;
-    if (r < top) out[r] = k;
-  }
-}
 
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_fwd(const __grid_constant__ FwdParams p) {
+__global__ void __launch_bounds__(kThreads, 5) token_logprobs_fwd(const __grid_constant__ FwdParams p) {
   constexpr int VEC = 16 / sizeof(T);
-  constexpr int UNROLL = 4;
   using V16 = Vec<T, VEC>;
   __shared__ Running warps[kThreads / 32];
   __shared__ Running all;
-  __shared__ TopShared ts;  // left out where TOP is false
   const int C = p.cluster, rank = blockIdx.x % C;
   const int64_t row = blockIdx.x / C;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
   const RowParts<T> parts(x, p.V);
   const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
   const int tid = threadIdx.x;
-  const int64_t step = (int64_t)kThreads * C, first = (int64_t)rank * kThreads + tid;
-
-  // one pass: vector j of the row belongs to thread j % (kThreads C) of the cluster
-  Fast sums = fast_start(p.c);
-  int64_t best_at = first;
-  auto take = [&](const V16& v, int64_t j) {
-    const float vm = largest<T>(v);
-    if (vm > sums.best) {
-      best_at = j;
-      fast_raise<ENT>(sums, vm, p.c);
-    }
-    fast_add<T, ENT>(sums, v, p.c);
-  };
-  int64_t j = first;
-  for (; j + (UNROLL - 1) * step < parts.vectors; j += UNROLL * step) {
-    V16 v[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) v[u] = xv[j + u * step];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) take(v[u], j + u * step);
+  int64_t token = -1;
+  float token_value = 0.f;
+  if (rank == 0 && tid == 0) {
+    token = p.tokens[row];
+    if (token >= 0 && token < p.V) token_value = to_f<T>(x[token]);
   }
-  for (; j < parts.vectors; j += step) take(xv[j], j);
+
+  // one pass, a tile of kTile vectors after the other: thread tid has vectors tid, tid + kThreads, ... of a tile
+  const int64_t tiles = (parts.vectors + kTile - 1) / kTile;
+  Fast sums = fast_start(p.c);
+  auto take = [&](const auto& v) {
+    const float vm = largest<T>(v);
+    sums.best = fmaxf(sums.best, vm);
+    if (vm > sums.limit) fast_raise<ENT>(sums, vm, p.c);
+#pragma unroll
+    for (const V16& u : v) fast_add<T, ENT>(sums, u, p.c);
+    return vm;
+  };
+  for (int64_t tile = rank; tile < tiles; tile += C) {
+    const int64_t j = tile * kTile + tid;
+    float most = -INFINITY;
+    if ((tile + 1) * kTile <= parts.vectors) {
+      V16 v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) v[u] = xv[j + u * kThreads];
+      most = fmaxf(most, take(v));
+    } else {
+      for (int u = 0; u < kUnroll; ++u) {
+        if (j + u * kThreads >= parts.vectors) break;
+        const V16 v[1] = {xv[j + u * kThreads]};
+        most = fmaxf(most, take(v));
+      }
+    }
+    if (TOP) {  // a group: the tile's vectors of 2^lanes_log neighbouring threads
+      const int lanes = 1 << p.lanes_log;
+      for (int o = 1; o < lanes; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if ((tid & (lanes - 1)) == 0)
+        p.maxima[((row * p.tiles + tile) * kThreads + tid) >> p.lanes_log] = most;
+    }
+  }
   Running a;
   if (!fast_done<T, ENT>(sums, p.c, a)) {
-    for (j = first; j < parts.vectors; j += step) {
-      float f[VEC];
-      widen(xv[j], f);
+    for (int64_t tile = rank; tile < tiles; tile += C) {
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t j = tile * kTile + u * kThreads + tid;
+        if (j >= parts.vectors) break;
+        float f[VEC];
+        widen(xv[j], f);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) add<ENT>(a, f[i], p.c);
+        for (int i = 0; i < VEC; ++i) add<ENT>(a, f[i], p.c);
+      }
     }
   }
   // the row's ends: at most 2 (VEC - 1) values, one each for the first threads of the cluster
-  const int64_t ends = parts.head + (p.V - parts.tail0);
-  const int64_t end_at = first < parts.head ? first : parts.tail0 + (first - parts.head);
-  if (first < ends) add<ENT>(a, to_f<T>(x[end_at]), p.c);
+  const int64_t end_at = tid < parts.head ? tid : parts.tail0 + (tid - parts.head);
+  if (rank == 0 && tid < parts.head + (p.V - parts.tail0)) add<ENT>(a, to_f<T>(x[end_at]), p.c);
 
   a = shuffle_join(a, p.c);
   if ((tid & 31) == 0) warps[tid >> 5] = a;
-  if constexpr (TOP) {
-    // the largest key of each group of 4 threads
-    long long k = kNoKey;
-    if (first < parts.vectors) {
-      const V16 v = xv[best_at];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) k = max(k, key_of(to_f<T>(v.v[i]), parts.head + best_at * VEC + i));
-    }
-    k = max(k, __shfl_xor_sync(0xffffffffu, k, 1));
-    k = max(k, __shfl_xor_sync(0xffffffffu, k, 2));
-    if ((tid & 3) == 0) ts.group[tid >> 2] = k;
-    if (tid == 0) {
-      ts.n_cand = ts.n_winners = 0;
-      ts.threshold = kNoKey;
-    }
-  }
   __syncthreads();
   if (tid < 32) {
     a = tid < kThreads / 32 ? warps[tid] : Running{kLowest, 0.f, 0.f};
     a = shuffle_join(a, p.c);
-    if (tid == 0) all = a;
-  }
-  if constexpr (TOP) {
-    if (tid < kGroups) {  // the k-th largest group maximum bounds the k-th largest value from below
-      const long long k = ts.group[tid];
-      int r = 0;
-      for (int i = 0; i < kGroups; ++i) r += ts.group[i] > k;
-      if (r == p.top - 1 && k != kNoKey) ts.threshold = k;
-    }
-    __syncthreads();
-    const long long threshold = ts.threshold;
-    if (tid < kGroups) {
-      const long long k = ts.group[tid];
-      if (k != kNoKey && k >= threshold) ts.winners[atomicAdd(&ts.n_winners, 1)] = tid;
-    }
-    __syncthreads();
-    const float floor_value = threshold == kNoKey ? -INFINITY : key_value(threshold);
-    auto offer = [&](float f, int64_t index) {
-      if (f < floor_value) return;
-      const long long k = key_of(f, index);
-      if (k < threshold) return;
-      const int at = atomicAdd(&ts.n_cand, 1);
-      if (at < kCandidates) ts.cand[at] = k;
-    };
-    // every vector of the winners: 4 threads each, one round of the first pass after the other
-    const unsigned won = ts.n_winners, rounds = (unsigned)((parts.vectors + step - 1) / step);
-    for (unsigned i = tid; i < rounds * 4 * won; i += kThreads) {
-      const unsigned round = i / 4 / won, owner = ts.winners[i / 4 - round * won] * 4 + (i & 3);
-      const int64_t jj = round * step + rank * kThreads + owner;
-      if (jj >= parts.vectors) continue;
-      const V16 v = xv[jj];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) offer(to_f<T>(v.v[e]), parts.head + jj * VEC + e);
-    }
-    if (first < ends) offer(to_f<T>(x[end_at]), end_at);
-    __syncthreads();
-    const int n = ts.n_cand;
-    if (n <= kCandidates) {
-      rank_keys(ts.cand, n, ts.best, p.top);
-    } else {
-      // More values above the bound than there is room for: rows whose largest values all lie in a few threads'
-      // vectors.  Takes the largest key below the last one, k times over.
-      long long last = LLONG_MAX;
-      for (int r = 0; r < p.top; ++r) {
-        long long k = kNoKey;
-        for (int64_t jj = first; jj < parts.vectors; jj += step) {
-          const V16 v = xv[jj];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const long long q = key_of(to_f<T>(v.v[e]), parts.head + jj * VEC + e);
-            if (q < last) k = max(k, q);
-          }
-        }
-        if (first < ends) {
-          const long long q = key_of(to_f<T>(x[end_at]), end_at);
-          if (q < last) k = max(k, q);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
-        __syncthreads();
-        if ((tid & 31) == 0) ts.red[tid >> 5] = k;
-        __syncthreads();
-        for (int w = 0; w < kThreads / 32; ++w) k = max(k, ts.red[w]);
-        if (tid == 0) ts.best[r] = k;
-        last = k;
-      }
-    }
   }
   if (C > 1) {  // the cluster's first CTA joins what the others hold
     cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) all = a;
     cluster.sync();
-    if (rank == 0) {
-      if (tid == 0) {
-        a = all;
-        for (int r = 1; r < C; ++r) join(a, *cluster.map_shared_rank(&all, r), p.c);
-      }
-      if constexpr (TOP) {
-        for (int i = tid; i < C * p.top; i += kThreads)
-          ts.cand[i] = *cluster.map_shared_rank(&ts.best[i % p.top], i / p.top);
-        __syncthreads();
-        rank_keys(ts.cand, C * p.top, ts.best, p.top);  // V >= top: every place is filled
-      }
+    if (rank == 0 && tid == 0) {
+      for (int r = 1; r < C; ++r) join(a, *cluster.map_shared_rank(&all, r), p.c);
     }
     cluster.sync();  // the others' shared memory lives until it has been read
-    if (rank != 0) return;
   }
-  if (TOP) __syncthreads();
+  if (rank != 0 || tid != 0) return;
+  // a row without any possible token has S = 0
+  const bool none = a.s == 0.f;
+  const float l2s = none ? -INFINITY : log2f(a.s);
+  float lp = 0.f;
+  if (token >= 0 && token < p.V) lp = none ? -INFINITY : (token_value - a.m) * p.inv_tau - l2s * kLn2;
+  p.logprob[row] = lp;
+  p.stats[2 * row] = a.m;
+  p.stats[2 * row + 1] = l2s;
+  if (ENT) p.entropy[row] = none ? 0.f : (l2s - a.w / a.s) * kLn2;
+}
+
+struct TopParams {
+  const void* logits;
+  const float* maxima;
+  const float* stats;
+  float* top_lp;
+  int64_t* top_ids;
+  int64_t ld, V, tiles;
+  float inv_tau;
+  int top, lanes_log;
+};
+
+struct TopShared {
+  int4 group[kSelThreads / 4];  // maxima of groups of columns
+  uint4 hit[kHits];             // vectors with a value from the bound on
+  int hit_at[kHits];
+  long long cand[kCandidates];
+  int winners[kMaxWinners];
+  int n_hit, n_cand, n_won, floor, larger;
+  long long threshold, red[kSelThreads / 32];
+};
+
+// Appends `column` to the winners where `win`.
+__device__ __forceinline__ void push_winner(TopShared& ts, bool win, int column) {
+  const unsigned all = __ballot_sync(0xffffffffu, win), lane = threadIdx.x & 31;
+  int base = 0;
+  if (lane == 0 && all != 0) base = atomicAdd(&ts.n_won, __popc(all));
+  const int at = __shfl_sync(0xffffffffu, base, 0) + __popc(all & ((1u << lane) - 1));
+  if (win && at < kMaxWinners) ts.winners[at] = column;
+}
+
+// One CTA per row. The groups c, c + kColumns, ... of the row are its column c; a thread looks after columns tid and
+// tid + kSelThreads.
+template <typename T>
+__global__ void __launch_bounds__(kSelThreads) token_logprobs_top(const __grid_constant__ TopParams p) {
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr unsigned kAll = 0xffffffffu;
+  using V16 = Vec<T, VEC>;
+  __shared__ TopShared ts;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+  const RowParts<T> parts(x, p.V);
+  const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
+  const int log = p.lanes_log;
+  const unsigned vectors = (unsigned)parts.vectors, groups = (vectors + kTile - 1) / kTile * (kThreads >> log);
+  int value[2] = {INT_MIN, INT_MIN};
+  int column_log = 2 + log;  // vectors of a column
+  static_assert(kUnroll == 4 && kThreads == 256, "the shifts here");
+  for (unsigned g = tid; g < groups; g += kColumns) {
+    const float* most = p.maxima + (row * p.tiles * kThreads >> log) + g;
+    value[0] = max(value[0], order_of(most[0]));
+    if (g + kSelThreads < groups) value[1] = max(value[1], order_of(most[kSelThreads]));
+  }
+  while ((unsigned)kColumns << (column_log - 2 - log) < groups) ++column_log;
+  // the r-th vector of a column, in the order of the row; `vectors` or more for none
+  auto vector_of = [&](unsigned column, unsigned r) {
+    const unsigned round = r >> log, g = column + (round >> 2) * kColumns, tile = g >> (8 - log);
+    return tile * kTile + (round & 3) * kThreads + ((g << log) & (kThreads - 1)) + (r & ((1u << log) - 1));
+  };
+  const float m = p.stats[2 * row], l2s = p.stats[2 * row + 1];
   if (tid == 0) {
-    all = a;
-    const int64_t t = p.tokens[row];
-    // a row without any possible token has S = 0
-    const bool none = a.s == 0.f;
-    const float l2s = none ? -INFINITY : log2f(a.s);
-    float lp = 0.f;
-    if (t >= 0 && t < p.V) lp = none ? -INFINITY : (to_f<T>(x[t]) - a.m) * p.inv_tau - l2s * kLn2;
-    p.logprob[row] = lp;
-    p.stats[2 * row] = a.m;
-    p.stats[2 * row + 1] = l2s;
-    if (ENT) p.entropy[row] = none ? 0.f : (l2s - a.w / a.s) * kLn2;
+    ts.n_hit = ts.n_cand = ts.n_won = ts.larger = 0;
+    ts.floor = INT_MAX;
+    ts.threshold = kNoKey;  // stays where fewer equal values are left than needed
   }
-  if constexpr (TOP) {
-    __syncthreads();
-    const float m = all.m, s = all.s;
-    const float l2s = s == 0.f ? -INFINITY : log2f(s);
-    for (int i = tid; i < p.top; i += kThreads) {
-      const int64_t id = key_index(ts.best[i]);
-      p.top_ids[row * p.top + i] = id;
-      p.top_lp[row * p.top + i] = s == 0.f ? -INFINITY : (to_f<T>(x[id]) - m) * p.inv_tau - l2s * kLn2;
+
+  // The bound: the k-th largest maximum of groups of 4 columns (64 groups, two threads for the comparisons of each), or
+  // for a larger k of 2 columns, which holds back more values.
+  int best = max(value[0], value[1]), above = 0;
+  const bool four = p.top <= 24;
+  if (four) best = max(best, __shfl_xor_sync(kAll, best, 1));
+  if (!four || (tid & 1) == 0) reinterpret_cast<int*>(ts.group)[four ? tid >> 1 : tid] = best;
+  __syncthreads();
+  {
+    const int n = four ? kSelThreads / 16 : kSelThreads / 4;
+    const int4* o = ts.group + (four ? (tid & 1) * n : 0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const int4 q = o[i];
+      above += (q.x > best) + (q.y > best) + (q.z > best) + (q.w > best);
     }
+    if (four) above += __shfl_xor_sync(kAll, above, 1);
+  }
+  const int low = __reduce_min_sync(kAll, best != INT_MIN && above < p.top ? best : INT_MAX);
+  const int full = __syncthreads_count(best != INT_MIN) >> (four ? 1 : 0);  // groups with values
+  if ((tid & 31) == 0) atomicMin(&ts.floor, low);
+  __syncthreads();
+  // with fewer groups than alternatives every value counts
+  int floor = full < p.top ? INT_MIN + 1 : ts.floor;
+  long long threshold = full < p.top ? kNoKey : (long long)floor * 0x100000000ll;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) push_winner(ts, value[i] >= floor, tid + i * kSelThreads);
+  __syncthreads();
+  int won = ts.n_won;
+  if (won > kMaxWinners) {
+    // Many columns share the bound (equal or masked logits), since fewer than kMaxWinners lie above it: of these, those
+    // with the lowest indexes win.
+    long long k[2] = {kNoKey, kNoKey};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int column = tid + i * kSelThreads;
+      if (value[i] == floor) {
+        for (unsigned q = 0; q >> column_log == 0 && k[i] == kNoKey; ++q) {
+          const unsigned j = vector_of(column, q);
+          if (j >= vectors) continue;
+          const V16 v = xv[j];
+#pragma unroll
+          for (int e = VEC - 1; e >= 0; --e) {
+            const float f = to_f<T>(v.v[e]);
+            if (order_of(f) == floor) k[i] = key_of(f, parts.head + (int64_t)j * VEC + e);
+          }
+        }
+      }
+      ts.cand[column] = k[i];
+      const unsigned more = __ballot_sync(kAll, value[i] > floor);
+      if ((tid & 31) == 0) atomicAdd(&ts.larger, __popc(more));
+    }
+    __syncthreads();
+    if (tid == 0) ts.n_won = 0;
+    const int need = p.top - ts.larger;  // so many of the equal ones
+    int r[2] = {0, 0};
+    for (int i = 0; i < kColumns; ++i) {
+      r[0] += ts.cand[i] > k[0];
+      r[1] += ts.cand[i] > k[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      push_winner(ts, value[i] > floor || (k[i] != kNoKey && r[i] < need), tid + i * kSelThreads);
+      if (k[i] != kNoKey && r[i] == need - 1) ts.threshold = k[i];
+    }
+    __syncthreads();
+    won = ts.n_won;
+    threshold = need > 0 ? ts.threshold : (long long)(floor + 1) * 0x100000000ll;
+  }
+
+  const float floor_value = threshold == kNoKey ? -INFINITY : key_value(threshold);
+  auto offer = [&](float f, int64_t index) {
+    if (f < floor_value) return;
+    const long long k = key_of(f, index);
+    if (k < threshold) return;
+    const int at = atomicAdd(&ts.n_cand, 1);
+    if (at < kCandidates) ts.cand[at] = k;
+  };
+  const int64_t last_equal = key_index(threshold);  // values that equal the bound count up to here
+  const unsigned todo = (unsigned)won << column_log;
+  for (unsigned i = tid; i < todo; i += kUnroll * kSelThreads) {
+    V16 v[kUnroll];
+    unsigned at[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const unsigned q = i + u * kSelThreads;
+      at[u] = q < todo ? vector_of(ts.winners[q >> column_log], q & ((1u << column_log) - 1)) : vectors;
+      if (at[u] < vectors) v[u] = xv[at[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (at[u] >= vectors) continue;
+      const V16 one[1] = {v[u]};
+      const float vm = largest<T>(one);
+      if (vm < floor_value || (vm == floor_value && parts.head + (int64_t)at[u] * VEC > last_equal)) continue;
+      const int h = atomicAdd(&ts.n_hit, 1);
+      if (h >= kHits) continue;
+      ts.hit[h] = *reinterpret_cast<const uint4*>(&v[u]);
+      ts.hit_at[h] = (int)at[u];
+    }
+  }
+  __syncthreads();
+  const int hits = ts.n_hit;
+  for (int i = tid; i < min(hits, kHits) * VEC; i += kSelThreads)
+    offer(to_f<T>(reinterpret_cast<const T*>(ts.hit)[i]), parts.head + (int64_t)ts.hit_at[i / VEC] * VEC + i % VEC);
+  // the row's ends, at most 2 (VEC - 1) values
+  const int64_t end_at = tid < parts.head ? tid : parts.tail0 + (tid - parts.head);
+  const bool end = end_at < p.V && tid < parts.head + (p.V - parts.tail0);
+  if (end) offer(to_f<T>(x[end_at]), end_at);
+  __syncthreads();
+
+  auto put = [&](int i, long long k) {
+    p.top_ids[row * p.top + i] = key_index(k);
+    p.top_lp[row * p.top + i] = l2s == -INFINITY ? -INFINITY : (key_value(k) - m) * p.inv_tau - l2s * kLn2;
+  };
+  const int n = ts.n_cand;
+  if (hits <= kHits && n <= kCandidates) {
+    // each candidate's place is the number of larger ones, which 4 threads count
+    const int part = tid & 3;
+    for (int i0 = 0; i0 < n; i0 += kSelThreads / 4) {
+      const int i = i0 + (tid >> 2);
+      const long long k = i < n ? ts.cand[i] : kNoKey;
+      int r = 0;
+#pragma unroll 4
+      for (int j = part; j < n; j += 4) r += ts.cand[j] > k;
+      r += __shfl_xor_sync(kAll, r, 1);
+      r += __shfl_xor_sync(kAll, r, 2);
+      if (part == 0 && i < n && r < p.top) put(r, k);
+    }
+    return;
+  }
+  // More values above the bound than there is room for: rows whose largest values all lie in a few columns. Takes the
+  // largest key below the last one, k times over.
+  long long last = LLONG_MAX;
+  for (int i = 0; i < p.top; ++i) {
+    long long k = kNoKey;
+    for (int64_t j = tid; j < parts.vectors; j += kSelThreads) {
+      const V16 v = xv[j];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const long long q = key_of(to_f<T>(v.v[e]), parts.head + j * VEC + e);
+        if (q < last) k = max(k, q);
+      }
+    }
+    if (end) {
+      const long long q = key_of(to_f<T>(x[end_at]), end_at);
+      if (q < last) k = max(k, q);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(kAll, k, o));
+    __syncthreads();
+    if ((tid & 31) == 0) ts.red[tid >> 5] = k;
+    __syncthreads();
+    for (int w = 0; w < kSelThreads / 32; ++w) k = max(k, ts.red[w]);
+    if (tid == 0) put(i, k);
+    last = k;
   }
 }
 
@@ -522,21 +655,25 @@ void token_logprobs_fwd_launch(const at::Tensor& logits, const at::Tensor& token
   p.logprob = logprob.data_ptr<float>();
   p.stats = stats.data_ptr<float>();
   if (entropy.defined()) p.entropy = entropy.data_ptr<float>();
-  if (top > 0) {
-    p.top_lp = top_lp.data_ptr<float>();
-    p.top_ids = top_ids.data_ptr<int64_t>();
-  }
   p.ld = rows > 1 ? logits.stride(0) : V;
   p.V = V;
   p.inv_tau = (float)inv_tau;
   p.c = (float)(inv_tau * 1.4426950408889634);
-  p.top = (int)top;
-  // clusters until every SM has work, as long as each thread has a vector to read
-  const int64_t vectors = V * logits.element_size() / 16;
+  const int64_t vectors = V * logits.element_size() / 16, tiles = std::max<int64_t>(1, (vectors + kTile - 1) / kTile);
+  p.tiles = tiles;
+  // groups small enough for at least 128 in a row, but no more than are looked at in one go
+  while (p.lanes_log < 5 && tiles * kThreads >> p.lanes_log > kColumns) ++p.lanes_log;
+  // Clusters while all CTAs are resident at once (5 on an SM) and each has a tile: 257 x 131072 fp32 45 us with one
+  // CTA for a row, 33 us with two, 37 us with four; 4 x 50304 bf16 6.6, 5.5, 4.7 and (eight) 4.2 us.
   int C = 1;
-  while (C < 8 && rows * C < num_sms() && vectors > (int64_t)kThreads * C) C *= 2;
+  while (C < 8 && rows * C * 2 <= 5 * num_sms() && tiles > C) C *= 2;
   p.cluster = C;
   MT_CHECK(rows * C < (int64_t(1) << 31), "token_logprobs: too many rows: ", rows);
+  at::Tensor maxima;
+  if (top > 0) {
+    maxima = at::Tensor(at::detail::empty_cuda({rows, tiles, kThreads >> p.lanes_log}, at::kFloat, logits.device(), c10::nullopt));
+    p.maxima = maxima.data_ptr<float>();
+  }
   auto launch = [&](auto kernel) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * C));
@@ -562,6 +699,11 @@ void token_logprobs_fwd_launch(const at::Tensor& logits, const at::Tensor& token
       launch(token_logprobs_fwd<T, false, true>);
     else
       launch(token_logprobs_fwd<T, false, false>);
+    if (top == 0) return;
+    TopParams q{p.logits, p.maxima, p.stats, top_lp.data_ptr<float>(), top_ids.data_ptr<int64_t>(), p.ld, V,
+                tiles, p.inv_tau, (int)top, p.lanes_log};
+    token_logprobs_top<T><<<(unsigned)rows, kSelThreads, 0, cur_stream()>>>(q);
+    MT_LAUNCH_CHECK();
   });
 }
 
