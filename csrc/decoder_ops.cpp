@@ -118,9 +118,9 @@ void check_pair(const at::Tensor& q, const at::Tensor& k) {
 }
 
 RotarySetup setup_of(const at::Tensor& turns, int64_t rot_dim, bool interleaved, double scale) {
-  TORCH_CHECK_VALUE(rot_dim > 0 && rot_dim % 2 == 0 && turns.scalar_type() == at::kDouble &&
+  TORCH_CHECK_VALUE(rot_dim > 0 && rot_dim % 2 == 0 && turns.scalar_type() == at::kLong &&
                         turns.is_contiguous() && turns.numel() == rot_dim / 2,
-                    "rotary: turns must hold rot_dim / 2 values in 64 bits");
+                    "rotary: turns must hold rot_dim / 2 fixed-point values");
   return RotarySetup{turns, rot_dim, interleaved, scale};
 }
 

@@ -18,7 +18,7 @@ struct RotarySegment {
   int64_t heads_rot;
 };
 struct RotaryArgs {
-  at::Tensor turns;  // fp64 [rot_dim / 2]: revolutions per position of each pair
+  at::Tensor turns;  // int64 [rot_dim / 2]: revolutions per position of each pair times 2^64, modulo 2^64
   int64_t rot_dim;
   bool interleaved;
   double scale;         // factor on the rotated values

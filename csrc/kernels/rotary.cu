@@ -2,12 +2,14 @@
 //   a' = s (a cos - b sin),  b' = s (a sin + b cos),
 // the rest of the head passes through; the backward is the same with -angle.
 //
-// Bound by memory: every value is read once and written once, with about 3 flops each.  One CTA takes a few
-// tokens and all their heads.  It computes the tokens' cosines and sines once, into shared memory (they are the
-// same for every head), then each thread owns one chunk of a head -- in the half layout VEC values of each half
-// -- and walks tokens and heads with 16-byte loads and stores.  No table is read: an angle is
-// pos * (w / 2 pi) revolutions in 64 bits, of which only the fraction goes on in 32 bits, so far positions
-// lose nothing and no longest length has to be set.
+// Bound by memory: every value is read once and written once, with about 3 flops each.  A thread owns one chunk of a
+// head -- in the half layout VEC values of each half -- of one token and takes it through several heads, 16-byte loads
+// and stores, as many tokens to a CTA as fill 256 threads.  It asks for its values first; while they are on their way
+// the CTA computes its tokens' cosines and sines, once for all heads, into shared memory.
+//
+// No table is read.  A frequency is a 64-bit fixed-point fraction of a revolution per position; times the position, modulo
+// 2^64, it is the angle without the whole revolutions, exact to |pos| 2^-65 of one (and 2^-53 of the angle from the
+// frequency itself).  So far positions lose nothing, no longest length has to be set, and no 64-bit floats are needed.
 #include "decoder_ops.h"
 #include "vec.cuh"
 
@@ -24,93 +26,114 @@ struct Seg {
 
 struct RotParams {
   Seg seg[2];
-  const double* turns;
+  const uint64_t* turns;
   const void* pos;
-  int64_t pos_b, pos_s, offset, S, tokens;
+  int64_t pos_b, pos_s, offset;
+  uint32_t S, tokens;
   int pos_size;  // bytes of a position; 0: offset + index in the sequence
-  int heads, half, chunks, rot_chunks, heads_per_pass, tile;
+  int heads, half, chunks, rot_chunks, pass_vectors, head_step, tile;
   float scale, sign;
   bool copy;  // out of place: values that are not rotated are copied
 };
 
-constexpr int kMaxThreads = 512;
 
-template <typename T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_constant__ RotParams p) {
-  extern __shared__ float2 cs[];  // [tile][half]
-  const int64_t t0 = (int64_t)blockIdx.x * p.tile;
-  const int nt = (int)min((int64_t)p.tile, p.tokens - t0);
-  for (int i = threadIdx.x; i < nt * p.half; i += blockDim.x) {
-    const int tt = i / p.half, pair = i - tt * p.half;
-    const int64_t t = t0 + tt, b = t / p.S, s = t - b * p.S;
-    int64_t pos = p.offset + s;
-    if (p.pos_size == 8) pos = static_cast<const int64_t*>(p.pos)[b * p.pos_b + s * p.pos_s];
-    if (p.pos_size == 4) pos = static_cast<const int32_t*>(p.pos)[b * p.pos_b + s * p.pos_s];
-    const double turn = (double)pos * p.turns[pair];
+// NV: vectors of a rotated chunk -- half a rotation apart, or (INTERLEAVED) neighbours.
+template <typename T, int VEC, bool INTERLEAVED, int NV, int U>
+__global__ void __launch_bounds__(VEC == 1 ? 512 : 256, VEC == 1 ? 1 : U == 2 ? 4 : 3) rotary_kernel(const __grid_constant__ RotParams p) {
+  extern __shared__ float2 cs[];  // [tokens of the CTA][half]
+  constexpr int NP = NV * VEC / 2;  // pairs of a chunk
+  using V = Vec<T, VEC>;
+  const uint32_t t0 = blockIdx.x * p.tile;
+  // thread = (token of the tile * head_step + first head) * chunks + chunk
+  const int row = threadIdx.x / p.chunks, c = threadIdx.x - row * p.chunks;
+  const int tt = row / p.head_step, first = row - tt * p.head_step;
+  const uint32_t t = t0 + tt, b = t / p.S, s = t - b * p.S;
+  const bool here = tt < p.tile && t < p.tokens, rot_chunk = c < p.rot_chunks;
+  const int pass_width = p.pass_vectors * VEC;
+  const int at = rot_chunk ? c * (INTERLEAVED ? NV * VEC : VEC) : 2 * p.half + (c - p.rot_chunks) * pass_width;
+  const int next = INTERLEAVED || !rot_chunk ? VEC : p.half;  // from a chunk's first vector to its second
+  const bool two = rot_chunk ? NV == 2 : p.pass_vectors == 2;
+
+  V x[U][2];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int hh = h0 + u * p.head_step;
+      const bool second = hh >= p.seg[0].heads;
+      const Seg& g = p.seg[second];
+      const int h = second ? hh - p.seg[0].heads : hh;
+      if (hh >= p.heads || !(p.copy || (rot_chunk && h < g.heads_rot))) continue;
+      const T* in = static_cast<const T*>(g.in) + b * g.in_b + s * g.in_s + h * g.in_h + at;
+      x[u][0] = load_stream(reinterpret_cast<const V*>(in));
+      if (two) x[u][1] = load_stream(reinterpret_cast<const V*>(in + next));
+    }
+  };
+  // The CTA's angles: thread i takes i, i + blockDim, ... of [token][pair]. Its first position is asked for before the
+  // values, behind which it would queue.
+  int ti = threadIdx.x / p.half, pair = threadIdx.x - ti * p.half;
+  const int dt = blockDim.x / p.half, dp = blockDim.x - dt * p.half;
+  auto position = [&](int ti) {
+    const uint32_t ta = min(t0 + ti, p.tokens - 1), ba = ta / p.S, sa = ta - ba * p.S;
+    if (p.pos_size == 8) return static_cast<const int64_t*>(p.pos)[ba * p.pos_b + sa * p.pos_s];
+    if (p.pos_size == 4) return (int64_t)static_cast<const int32_t*>(p.pos)[ba * p.pos_b + sa * p.pos_s];
+    return p.offset + sa;
+  };
+  int64_t pos = position(ti);
+  uint64_t turns = p.turns[pair];
+  if (here) load(first);
+  while (ti < p.tile) {
+    const uint64_t turn = (uint64_t)pos * turns;
     float sn, cn;
-    sincospif(2.f * (float)(turn - rint(turn)), &sn, &cn);
-    cs[i] = make_float2(cn * p.scale, sn * p.scale * p.sign);
+    sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &sn, &cn);
+    cs[ti * p.half + pair] = make_float2(cn * p.scale, sn * p.scale * p.sign);
+    ti += dt;
+    pair += dp;
+    if (pair >= p.half) {
+      pair -= p.half;
+      ++ti;
+    }
+    if (ti < p.tile) {
+      pos = position(ti);
+      turns = p.turns[pair];
+    }
   }
   __syncthreads();
-  const int hp = threadIdx.x / p.chunks, c = threadIdx.x - hp * p.chunks;
-  if (hp >= p.heads_per_pass) return;
-  // A chunk: two vectors half a rotation apart, or 1-2 vectors of neighbouring pairs.  NV vectors, NP pairs.
-  constexpr int NV = INTERLEAVED ? (VEC == 1 ? 2 : 1) : 2;
-  constexpr int NP = NV * VEC / 2;
-  constexpr int U = INTERLEAVED ? 4 : 2;  // heads in flight per thread
-  using V = Vec<T, VEC>;
-  const bool rot_chunk = c < p.rot_chunks;
-  const int at = rot_chunk ? (INTERLEAVED ? c * NV * VEC : c * VEC) : 2 * p.half + (c - p.rot_chunks) * VEC;
-  const int next = INTERLEAVED ? VEC : p.half;  // from a chunk's first vector to its second
-  for (int tt = 0; tt < nt; ++tt) {
-    const int64_t t = t0 + tt, b = t / p.S, s = t - b * p.S;
-    float cn[NP], sn[NP];
-    if (rot_chunk) {
+  if (!here) return;
+  float cn[NP], sn[NP];
+  if (rot_chunk) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const float2 v = cs[tt * p.half + c * NP + i];
-        cn[i] = v.x;
-        sn[i] = v.y;
-      }
+    for (int i = 0; i < NP; ++i) {
+      const float2 v = cs[tt * p.half + c * NP + i];
+      cn[i] = v.x;
+      sn[i] = v.y;
     }
-    for (int h0 = hp; h0 < p.heads; h0 += U * p.heads_per_pass) {
-      V x[U][NV];
-      T* out[U];
-      bool turned[U], todo[U];
+  }
+  for (int h0 = first; h0 < p.heads; h0 += U * p.head_step) {
+    if (h0 != first) load(h0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int hh = h0 + u * p.heads_per_pass;
-        const bool second = hh >= p.seg[0].heads;
-        const Seg& g = p.seg[second];
-        const int h = second ? hh - p.seg[0].heads : hh;
-        const T* in = static_cast<const T*>(g.in) + b * g.in_b + s * g.in_s + h * g.in_h + at;
-        out[u] = static_cast<T*>(g.out) + b * g.out_b + s * g.out_s + h * g.out_h + at;
-        turned[u] = rot_chunk && h < g.heads_rot;
-        todo[u] = hh < p.heads && (turned[u] || p.copy);
-        if (todo[u]) {
-          x[u][0] = load_stream(reinterpret_cast<const V*>(in));
-          if (NV == 2 && rot_chunk) x[u][NV - 1] = load_stream(reinterpret_cast<const V*>(in + next));
+    for (int u = 0; u < U; ++u) {
+      const int hh = h0 + u * p.head_step;
+      const bool second = hh >= p.seg[0].heads;
+      const Seg& g = p.seg[second];
+      const int h = second ? hh - p.seg[0].heads : hh;
+      const bool turned = rot_chunk && h < g.heads_rot;
+      if (hh >= p.heads || !(p.copy || turned)) continue;
+      if (turned) {
+        float f[NV * VEC], r[NV * VEC];
+        widen(x[u][0], f);
+        if (NV == 2) widen(x[u][1], f + (NV - 1) * VEC);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int ia = INTERLEAVED ? 2 * i : i, ib = INTERLEAVED ? 2 * i + 1 : VEC + i;
+          r[ia] = f[ia] * cn[i] - f[ib] * sn[i];
+          r[ib] = f[ia] * sn[i] + f[ib] * cn[i];
         }
+        x[u][0] = narrow<T, VEC>(r);
+        if (NV == 2) x[u][1] = narrow<T, VEC>(r + (NV - 1) * VEC);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!todo[u]) continue;
-        if (turned[u]) {
-          float f[NV * VEC], r[NV * VEC];
-          widen(x[u][0], f);
-          if (NV == 2) widen(x[u][NV - 1], f + (NV - 1) * VEC);
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            const int ia = INTERLEAVED ? 2 * i : i, ib = INTERLEAVED ? 2 * i + 1 : VEC + i;
-            r[ia] = f[ia] * cn[i] - f[ib] * sn[i];
-            r[ib] = f[ia] * sn[i] + f[ib] * cn[i];
-          }
-          x[u][0] = narrow<T, VEC>(r);
-          if (NV == 2) x[u][NV - 1] = narrow<T, VEC>(r + (NV - 1) * VEC);
-        }
-        store_stream(reinterpret_cast<V*>(out[u]), x[u][0]);
-        if (NV == 2 && rot_chunk) store_stream(reinterpret_cast<V*>(out[u] + next), x[u][NV - 1]);
-      }
+      T* out = static_cast<T*>(g.out) + b * g.out_b + s * g.out_s + h * g.out_h + at;
+      store_stream(reinterpret_cast<V*>(out), x[u][0]);
+      if (two) store_stream(reinterpret_cast<V*>(out + next), x[u][1]);
     }
   }
 }
@@ -130,20 +153,30 @@ int widest_vector(const RotParams& p, int nseg, int64_t D, int esize, bool inter
   return 1;
 }
 
-template <typename T, int VEC, bool IL>
-void launch(RotParams p, int64_t D) {
-  p.rot_chunks = IL ? 2 * p.half / (VEC == 1 ? 2 : VEC) : p.half / VEC;
-  p.chunks = p.rot_chunks + (int)(D - 2 * p.half) / VEC;
-  // the heads split evenly over the passes of a block of about 256 threads
-  const int fit = std::max(1, 256 / p.chunks);
-  const int passes = (p.heads + fit - 1) / fit;
-  p.heads_per_pass = (p.heads + passes - 1) / passes;
-  const int threads = (p.heads_per_pass * p.chunks + 31) / 32 * 32;
-  p.tile = p.tokens >= 4 * 1024 ? 4 : 1;
-  const int64_t blocks = (p.tokens + p.tile - 1) / p.tile;
-  MT_CHECK(blocks < (int64_t(1) << 31), "rotary: too many tokens: ", p.tokens);
-  rotary_kernel<T, VEC, IL><<<(unsigned)blocks, threads, (size_t)p.tile * p.half * sizeof(float2), cur_stream()>>>(p);
+// With U heads in flight per thread; false, and nothing launched, where that leaves SMs without work.
+template <typename T, int VEC, bool IL, int NV, int U>
+bool try_launch(RotParams p, int64_t D) {
+  const int rest = (int)(D - 2 * p.half) / VEC;  // vectors that pass through
+  p.pass_vectors = rest % 2 == 0 ? 2 : 1;
+  p.rot_chunks = 2 * p.half / (NV * VEC);
+  p.chunks = p.rot_chunks + rest / p.pass_vectors;
+  // threads of a token: enough to take all heads at once, in a CTA of about 256 threads
+  p.head_step = std::max(1, std::min((p.heads + U - 1) / U, 256 / p.chunks));
+  const int per_token = p.head_step * p.chunks;
+  p.tile = std::max(1, std::min(256 / per_token, 4096 / p.half));  // up to 32 KB of cosines and sines
+  const int threads = (per_token * p.tile + 31) / 32 * 32;
+  const unsigned blocks = (p.tokens + p.tile - 1) / p.tile;
+  if (U == 4 && blocks < 4u * num_sms()) return false;
+  rotary_kernel<T, VEC, IL, NV, U><<<blocks, threads, (size_t)p.tile * p.half * sizeof(float2), cur_stream()>>>(p);
   MT_LAUNCH_CHECK();
+  return true;
+}
+
+// Four heads where there are many tokens (8 x 2048 tokens of 48 heads x 128 bf16: 62 - 65 us, with two 75 us), two for few
+// (500 tokens of 20 heads x 128: 3.6 us, with four 3.9 us; 8 tokens of 40 heads 2.6 us and 3.3 us).
+template <typename T, int VEC, bool IL, int NV>
+void launch(const RotParams& p, int64_t D) {
+  if (!try_launch<T, VEC, IL, NV, 4>(p, D)) try_launch<T, VEC, IL, NV, 2>(p, D);
 }
 
 }  // namespace
@@ -160,10 +193,11 @@ void rotary_launch(const std::vector<RotarySegment>& segs, const RotaryArgs& a) 
                    (int)in.size(2),   (int)segs[i].heads_rot};
     p.heads += (int)in.size(2);
   }
-  p.turns = a.turns.data_ptr<double>();
+  p.turns = reinterpret_cast<const uint64_t*>(a.turns.data_ptr<int64_t>());
   p.half = (int)(a.rot_dim / 2);
-  p.S = S;
-  p.tokens = B * S;
+  MT_CHECK(B * S < (int64_t(1) << 31), "rotary: too many tokens: ", B * S);
+  p.S = (uint32_t)S;
+  p.tokens = (uint32_t)(B * S);
   p.offset = a.offset;
   if (a.positions.has_value()) {
     p.pos = a.positions->data_ptr();
@@ -178,19 +212,23 @@ void rotary_launch(const std::vector<RotarySegment>& segs, const RotaryArgs& a) 
   dispatch_act(segs[0].in.scalar_type(), [&](auto t) {
     using T = decltype(t);
     const int v = widest_vector(p, (int)segs.size(), D, sizeof(T), a.interleaved);
-    auto go = [&](auto il) {
+    auto go = [&](auto il, auto nv) {
       constexpr bool IL = decltype(il)::value;
+      constexpr int NV = decltype(nv)::value;
       if constexpr (sizeof(T) == 2) {
-        if (v == 8) return launch<T, 8, IL>(p, D);
+        if (v == 8) return launch<T, 8, IL, NV>(p, D);
       }
-      if (v == 4) return launch<T, 4, IL>(p, D);
-      if (v == 2) return launch<T, 2, IL>(p, D);
-      launch<T, 1, IL>(p, D);
+      if (v == 4) return launch<T, 4, IL, NV>(p, D);
+      if (v == 2) return launch<T, 2, IL, NV>(p, D);
+      launch<T, 1, IL, 2>(p, D);
     };
-    if (a.interleaved)
-      go(std::true_type{});
+    using two = std::integral_constant<int, 2>;
+    if (!a.interleaved)
+      go(std::false_type{}, two{});
+    else if (a.rot_dim % (2 * v) == 0)
+      go(std::true_type{}, two{});
     else
-      go(std::false_type{});
+      go(std::true_type{}, std::integral_constant<int, 1>{});
   });
 }
 

@@ -30,6 +30,9 @@ def build_inplace(quiet: bool = True) -> None:
 
 
 def _load(name: str):
+    mod = _mods.get(name)
+    if mod is not None:
+        return mod
     with _lock:
         if name in _mods:
             return _mods[name]

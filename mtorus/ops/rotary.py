@@ -2,7 +2,7 @@
 
 Each pair of a head's first ``rot_dim`` values turns by position x frequency:
 (a, b) -> s (a cos - b sin, a sin + b cos).  The kernel (``csrc/kernels/rotary.cu``)
-computes the angles itself, in 64 bits, from the positions and ``rot_dim / 2``
+computes the angles itself, in 64-bit fixed point, from the positions and ``rot_dim / 2``
 frequencies, so there is no table and no longest position.
 
     rope = RotaryPositions(128, scaling="yarn", factor=8, original_len=2048, device="cuda")
@@ -18,8 +18,8 @@ with any strides (rows that are not dense in the head dim are copied first), hea
 dim at most 512; results are computed in fp32 and rounded once.  ``positions`` is
 int64 or int32, [tokens], [batch, tokens] or [1, tokens] ([batch] too, for one token
 per sequence); without it token i of a sequence has position ``offset + i``.
-Positions are read on the device and may be any integer, negative ones included;
-beyond 2^53 / rot_dim or so angles lose their meaning.
+Positions are read on the device and may be any integer, negative ones included; an
+angle is as exact as its frequency in 64 bits (2^-53 of it).
 
 A CUDA graph that records the backward must be the only holder of an autograd
 graph of its leaves: drop eager results of the same leaves before the capture.
@@ -95,8 +95,9 @@ class RotaryPositions:
         if not math.isfinite(self.scale):
             raise ValueError("attention_scale must be finite")
         self.frequencies = freq
-        # revolutions per position, in 64 bits
-        self.turns = torch.tensor([w / (2.0 * math.pi) for w in freq], dtype=torch.float64, device=device)
+        # revolutions per position as 64-bit fixed-point fractions (the bits of a uint64)
+        turns = [int(w / (2.0 * math.pi) * 2.0 ** 64) for w in freq]
+        self.turns = torch.tensor([t - (t >> 63 << 64) for t in turns], dtype=torch.int64, device=device)
         self.args = (self.turns, self.rot_dim, layout == "interleaved", self.scale)
 
     def _check(self, dim: int) -> None:

@@ -47,7 +47,8 @@ def test_rotary_frequencies():
         if t < 0.8:
             assert f == x / 8
     assert _rope(rot_dim=2, scaling="ntk", factor=4).frequencies == [1.0]
-    assert torch.equal(_rope().turns, torch.tensor(w, dtype=torch.float64) / (2 * math.pi))
+    for t, x in zip(_rope().turns.tolist(), w):  # 64-bit fixed-point fractions of a revolution
+        assert abs(t / 2.0 ** 64 - x / (2 * math.pi)) <= 2.0 ** -53 * x + 2.0 ** -64
 
 
 def test_rotary_refuses():
