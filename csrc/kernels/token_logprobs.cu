@@ -30,10 +30,9 @@ namespace {
 
 constexpr int kThreads = 256;  // of a CTA of the first pass and of the backward
 constexpr int kUnroll = 4;     // vectors of a thread in flight
-constexpr int kTile = kThreads * kUnroll;
 constexpr int kSelThreads = 128;
 constexpr int kColumns = 2 * kSelThreads;
-constexpr int kMaxWinners = 128;
+constexpr int kManyWinners = 128;
 constexpr int kMaxTop = 64;
 constexpr int kHits = 512, kCandidates = 768;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -233,28 +232,49 @@ struct RowParts {
   }
 };
 
+// How the first kernel's maxima cut up a row for the second. A tile is kUnroll vectors for each of 2^threads_log threads,
+// thread i's being i, i + 2^threads_log, ...; a group is the vectors of 2^lanes_log neighbouring threads in a tile, or
+// (single) one vector.
+struct Groups {
+  uint32_t stride;  // groups of the row with the most
+  int threads_log, lanes_log;
+  bool single;
+};
+
+// All values -inf: what a thread without a vector takes in its place.
+template <typename T>
+__device__ __forceinline__ Vec<T, 16 / sizeof(T)> masked_vector() {
+  const uint32_t w = std::is_same_v<T, bf16> ? 0xff80ff80u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff800000u;
+  const uint4 v = make_uint4(w, w, w, w);
+  return *reinterpret_cast<const Vec<T, 16 / sizeof(T)>*>(&v);
+}
+
 struct FwdParams {
   const void* logits;
   const int64_t* tokens;
   float *logprob, *stats, *entropy;
-  float* maxima;  // [rows, tiles, kThreads >> lanes_log], or nullptr; -inf for a group without values
-  int64_t ld, V, tiles;  // tiles: of the row with the most
+  float* maxima;  // [rows, groups], or nullptr; -inf for a group without values
+  int64_t rows, ld, V;
   float c, inv_tau;
-  int cluster, lanes_log;
+  int cluster;
+  Groups groups;
 };
 
-template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kThreads, 5) token_logprobs_fwd(const __grid_constant__ FwdParams p) {
-  constexpr int VEC = 16 / sizeof(T);
+// NT: threads that share a row, a CTA (or one of a cluster) or a warp.
+template <typename T, bool ENT, bool TOP, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : 5) token_logprobs_fwd(const __grid_constant__ FwdParams p) {
+  constexpr int VEC = 16 / sizeof(T), TILE = NT * kUnroll;
+  constexpr bool WARP = NT == 32;
   using V16 = Vec<T, VEC>;
   __shared__ Running warps[kThreads / 32];
   __shared__ Running all;
-  const int C = p.cluster, rank = blockIdx.x % C;
-  const int64_t row = blockIdx.x / C;
+  const int C = WARP ? 1 : p.cluster, rank = WARP ? 0 : blockIdx.x % C;
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5) : blockIdx.x / C;
+  if (WARP && row >= p.rows) return;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
   const RowParts<T> parts(x, p.V);
   const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
-  const int tid = threadIdx.x;
   int64_t token = -1;
   float token_value = 0.f;
   if (rank == 0 && tid == 0) {
@@ -262,10 +282,10 @@ __global__ void __launch_bounds__(kThreads, 5) token_logprobs_fwd(const __grid_c
     if (token >= 0 && token < p.V) token_value = to_f<T>(x[token]);
   }
 
-  // one pass, a tile of kTile vectors after the other: thread tid has vectors tid, tid + kThreads, ... of a tile
-  const int64_t tiles = (parts.vectors + kTile - 1) / kTile;
+  // one pass, a tile after the other
+  const int64_t tiles = (parts.vectors + TILE - 1) / TILE;
   Fast sums = fast_start(p.c);
-  auto take = [&](const auto& v) {
+  auto take = [&](const auto& v) {  // the values of one or more vectors; their maximum
     const float vm = largest<T>(v);
     sums.best = fmaxf(sums.best, vm);
     if (vm > sums.limit) fast_raise<ENT>(sums, vm, p.c);
@@ -273,33 +293,49 @@ __global__ void __launch_bounds__(kThreads, 5) token_logprobs_fwd(const __grid_c
     for (const V16& u : v) fast_add<T, ENT>(sums, u, p.c);
     return vm;
   };
-  for (int64_t tile = rank; tile < tiles; tile += C) {
-    const int64_t j = tile * kTile + tid;
-    float most = -INFINITY;
-    if ((tile + 1) * kTile <= parts.vectors) {
-      V16 v[kUnroll];
+  auto keep = [&](const V16(&v)[kUnroll], int64_t tile, float vm) {  // the tile's maxima
+    float* most = p.maxima + row * p.groups.stride;
+    if (WARP && p.groups.single) {
+      const int64_t j = tile * TILE + tid;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) v[u] = xv[j + u * kThreads];
-      most = fmaxf(most, take(v));
-    } else {
       for (int u = 0; u < kUnroll; ++u) {
-        if (j + u * kThreads >= parts.vectors) break;
-        const V16 v[1] = {xv[j + u * kThreads]};
-        most = fmaxf(most, take(v));
+        const V16 one[1] = {v[u]};
+        if (j + u * NT < parts.vectors) most[j + u * NT] = fmaxf(-INFINITY, largest<T>(one));
       }
+    } else {
+      const int lanes = 1 << p.groups.lanes_log;
+      vm = fmaxf(-INFINITY, vm);
+      for (int o = 1; o < lanes; o *= 2) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+      if ((tid & (lanes - 1)) == 0) most[(tile * NT + tid) >> p.groups.lanes_log] = vm;
     }
-    if (TOP) {  // a group: the tile's vectors of 2^lanes_log neighbouring threads
-      const int lanes = 1 << p.lanes_log;
-      for (int o = 1; o < lanes; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if ((tid & (lanes - 1)) == 0)
-        p.maxima[((row * p.tiles + tile) * kThreads + tid) >> p.lanes_log] = most;
+  };
+  int64_t tile = rank;
+  for (; (tile + 1) * TILE <= parts.vectors; tile += C) {
+    const V16* from = xv + tile * TILE + tid;
+    V16 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = from[u * NT];
+    const float vm = take(v);
+    if constexpr (TOP) keep(v, tile, vm);
+  }
+  if (tile < tiles) {  // the last one, where it is not full
+    const int64_t j = tile * TILE + tid;
+    V16 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = j + u * NT < parts.vectors ? xv[j + u * NT] : masked_vector<T>();
+    float vm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const V16 one[1] = {v[u]};
+      if (tile * TILE + u * NT < parts.vectors) vm = fmaxf(vm, take(one));
     }
+    if constexpr (TOP) keep(v, tile, vm);
   }
   Running a;
   if (!fast_done<T, ENT>(sums, p.c, a)) {
-    for (int64_t tile = rank; tile < tiles; tile += C) {
+    for (tile = rank; tile < tiles; tile += C) {
       for (int u = 0; u < kUnroll; ++u) {
-        const int64_t j = tile * kTile + u * kThreads + tid;
+        const int64_t j = tile * TILE + u * NT + tid;
         if (j >= parts.vectors) break;
         float f[VEC];
         widen(xv[j], f);
@@ -308,25 +344,27 @@ __global__ void __launch_bounds__(kThreads, 5) token_logprobs_fwd(const __grid_c
       }
     }
   }
-  // the row's ends: at most 2 (VEC - 1) values, one each for the first threads of the cluster
+  // the row's ends: at most 2 (VEC - 1) values, one each for the first threads of the row
   const int64_t end_at = tid < parts.head ? tid : parts.tail0 + (tid - parts.head);
   if (rank == 0 && tid < parts.head + (p.V - parts.tail0)) add<ENT>(a, to_f<T>(x[end_at]), p.c);
 
   a = shuffle_join(a, p.c);
-  if ((tid & 31) == 0) warps[tid >> 5] = a;
-  __syncthreads();
-  if (tid < 32) {
-    a = tid < kThreads / 32 ? warps[tid] : Running{kLowest, 0.f, 0.f};
-    a = shuffle_join(a, p.c);
-  }
-  if (C > 1) {  // the cluster's first CTA joins what the others hold
-    cg::cluster_group cluster = cg::this_cluster();
-    if (tid == 0) all = a;
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
-      for (int r = 1; r < C; ++r) join(a, *cluster.map_shared_rank(&all, r), p.c);
+  if constexpr (!WARP) {
+    if ((tid & 31) == 0) warps[tid >> 5] = a;
+    __syncthreads();
+    if (tid < 32) {
+      a = tid < kThreads / 32 ? warps[tid] : Running{kLowest, 0.f, 0.f};
+      a = shuffle_join(a, p.c);
     }
-    cluster.sync();  // the others' shared memory lives until it has been read
+    if (C > 1) {  // the cluster's first CTA joins what the others hold
+      cg::cluster_group cluster = cg::this_cluster();
+      if (tid == 0) all = a;
+      cluster.sync();
+      if (rank == 0 && tid == 0) {
+        for (int r = 1; r < C; ++r) join(a, *cluster.map_shared_rank(&all, r), p.c);
+      }
+      cluster.sync();  // the others' shared memory lives until it has been read
+    }
   }
   if (rank != 0 || tid != 0) return;
   // a row without any possible token has S = 0
@@ -346,17 +384,18 @@ struct TopParams {
   const float* stats;
   float* top_lp;
   int64_t* top_ids;
-  int64_t ld, V, tiles;
+  int64_t ld, V;
   float inv_tau;
-  int top, lanes_log;
+  int top;
+  Groups groups;
 };
 
 struct TopShared {
-  int4 group[kSelThreads / 4];  // maxima of groups of columns
+  int4 group[kColumns / 4];  // maxima of columns, or of a few together
   uint4 hit[kHits];             // vectors with a value from the bound on
   int hit_at[kHits];
   long long cand[kCandidates];
-  int winners[kMaxWinners];
+  int winners[kColumns];
   int n_hit, n_cand, n_won, floor, larger;
   long long threshold, red[kSelThreads / 32];
 };
@@ -367,7 +406,7 @@ __device__ __forceinline__ void push_winner(TopShared& ts, bool win, int column)
   int base = 0;
   if (lane == 0 && all != 0) base = atomicAdd(&ts.n_won, __popc(all));
   const int at = __shfl_sync(0xffffffffu, base, 0) + __popc(all & ((1u << lane) - 1));
-  if (win && at < kMaxWinners) ts.winners[at] = column;
+  if (win) ts.winners[at] = column;
 }
 
 // One CTA per row. The groups c, c + kColumns, ... of the row are its column c; a thread looks after columns tid and
@@ -383,21 +422,31 @@ __global__ void __launch_bounds__(kSelThreads) token_logprobs_top(const __grid_c
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
   const RowParts<T> parts(x, p.V);
   const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
-  const int log = p.lanes_log;
-  const unsigned vectors = (unsigned)parts.vectors, groups = (vectors + kTile - 1) / kTile * (kThreads >> log);
+  static_assert(kUnroll == 4, "the shifts here");
+  const int log = p.groups.lanes_log, threads_log = p.groups.threads_log;
+  const bool single = p.groups.single;
+  const unsigned vectors = (unsigned)parts.vectors;
+  const unsigned full = vectors >> (threads_log + 2), rest = vectors - (full << (threads_log + 2));  // tiles, vectors
+  const unsigned groups = single ? vectors : (full + (rest != 0)) << (threads_log - log);
+  // groups with values, and the columns that hold them
+  const unsigned real = single ? vectors
+                               : (full << (threads_log - log)) + ((min(rest, 1u << threads_log) + (1u << log) - 1) >> log);
+  const int columns = (int)min(real, (unsigned)kColumns);
   int value[2] = {INT_MIN, INT_MIN};
-  int column_log = 2 + log;  // vectors of a column
-  static_assert(kUnroll == 4 && kThreads == 256, "the shifts here");
   for (unsigned g = tid; g < groups; g += kColumns) {
-    const float* most = p.maxima + (row * p.tiles * kThreads >> log) + g;
+    const float* most = p.maxima + row * p.groups.stride + g;
     value[0] = max(value[0], order_of(most[0]));
     if (g + kSelThreads < groups) value[1] = max(value[1], order_of(most[kSelThreads]));
   }
-  while ((unsigned)kColumns << (column_log - 2 - log) < groups) ++column_log;
+  int column_log = single ? 0 : 2 + log;  // vectors of a column
+  const int group_log = column_log;
+  while ((unsigned)kColumns << (column_log - group_log) < groups) ++column_log;
   // the r-th vector of a column, in the order of the row; `vectors` or more for none
   auto vector_of = [&](unsigned column, unsigned r) {
-    const unsigned round = r >> log, g = column + (round >> 2) * kColumns, tile = g >> (8 - log);
-    return tile * kTile + (round & 3) * kThreads + ((g << log) & (kThreads - 1)) + (r & ((1u << log) - 1));
+    if (single) return column + r * kColumns;
+    const unsigned round = r >> log, g = column + (round >> 2) * kColumns, tile = g >> (threads_log - log);
+    return (tile << (threads_log + 2)) + ((round & 3) << threads_log) +
+           ((g << log) & ((1u << threads_log) - 1)) + (r & ((1u << log) - 1));
   };
   const float m = p.stats[2 * row], l2s = p.stats[2 * row + 1];
   if (tid == 0) {
@@ -406,14 +455,33 @@ __global__ void __launch_bounds__(kSelThreads) token_logprobs_top(const __grid_c
     ts.threshold = kNoKey;  // stays where fewer equal values are left than needed
   }
 
-  // The bound: the k-th largest maximum of groups of 4 columns (64 groups, two threads for the comparisons of each), or
-  // for a larger k of 2 columns, which holds back more values.
-  int best = max(value[0], value[1]), above = 0;
-  const bool four = p.top <= 24;
-  if (four) best = max(best, __shfl_xor_sync(kAll, best, 1));
-  if (!four || (tid & 1) == 0) reinterpret_cast<int*>(ts.group)[four ? tid >> 1 : tid] = best;
-  __syncthreads();
-  {
+  // The bound: the k-th largest of the columns' maxima, or, where there are many more columns than that, of the maxima of
+  // 2 or 4 columns: fewer comparisons, shared by two threads for 4 columns, for a few more values to rank.
+  const int merged = columns >= 6 * p.top ? 4 : columns >= 3 * p.top ? 2 : 1;
+  int low = INT_MAX;  // smallest maximum that fewer than k others exceed
+  if (merged == 1) {
+    int* list = reinterpret_cast<int*>(ts.group);
+    list[tid] = value[0];
+    list[tid + kSelThreads] = value[1];
+    __syncthreads();
+    int above[2] = {0, 0};
+#pragma unroll 4
+    for (int i = 0; i < kColumns / 4; ++i) {
+      const int4 q = ts.group[i];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        above[k] += (q.x > value[k]) + (q.y > value[k]) + (q.z > value[k]) + (q.w > value[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (value[k] != INT_MIN && above[k] < p.top) low = min(low, value[k]);
+    }
+  } else {
+    const bool four = merged == 4;
+    int best = max(value[0], value[1]), above = 0;
+    if (four) best = max(best, __shfl_xor_sync(kAll, best, 1));
+    if (!four || (tid & 1) == 0) reinterpret_cast<int*>(ts.group)[four ? tid >> 1 : tid] = best;
+    __syncthreads();
     const int n = four ? kSelThreads / 16 : kSelThreads / 4;
     const int4* o = ts.group + (four ? (tid & 1) * n : 0);
 #pragma unroll 8
@@ -422,21 +490,20 @@ __global__ void __launch_bounds__(kSelThreads) token_logprobs_top(const __grid_c
       above += (q.x > best) + (q.y > best) + (q.z > best) + (q.w > best);
     }
     if (four) above += __shfl_xor_sync(kAll, above, 1);
+    if (best != INT_MIN && above < p.top) low = best;
   }
-  const int low = __reduce_min_sync(kAll, best != INT_MIN && above < p.top ? best : INT_MAX);
-  const int full = __syncthreads_count(best != INT_MIN) >> (four ? 1 : 0);  // groups with values
+  low = __reduce_min_sync(kAll, low);
   if ((tid & 31) == 0) atomicMin(&ts.floor, low);
   __syncthreads();
-  // with fewer groups than alternatives every value counts
-  int floor = full < p.top ? INT_MIN + 1 : ts.floor;
-  long long threshold = full < p.top ? kNoKey : (long long)floor * 0x100000000ll;
+  // with fewer columns than alternatives every value counts
+  const int floor = columns < p.top ? INT_MIN + 1 : ts.floor;
+  long long threshold = columns < p.top ? kNoKey : (long long)floor * 0x100000000ll;
 #pragma unroll
   for (int i = 0; i < 2; ++i) push_winner(ts, value[i] >= floor, tid + i * kSelThreads);
   __syncthreads();
   int won = ts.n_won;
-  if (won > kMaxWinners) {
-    // Many columns share the bound (equal or masked logits), since fewer than kMaxWinners lie above it: of these, those
-    // with the lowest indexes win.
+  if (won > kManyWinners) {
+    // Many columns share the bound (equal or masked logits): of these, those with the lowest indexes win.
     long long k[2] = {kNoKey, kNoKey};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -570,18 +637,21 @@ struct BwdParams {
   void* dlogits;
   const int64_t *tokens, *top_ids;
   const float *stats, *entropy, *g_logprob, *g_entropy, *g_top;
-  int64_t ld, V;
+  int64_t rows, ld, V;
   float c, inv_tau;
   int top, splits;
 };
 
-// One CTA per row, or per one of `splits` parts of a row.
-template <typename T, bool ENT>
+// NT threads share a row: a CTA, or one of `splits` for parts of the row, or a warp.
+template <typename T, bool ENT, int NT>
 __global__ void __launch_bounds__(kThreads) token_logprobs_bwd(const __grid_constant__ BwdParams p) {
   constexpr int VEC = 16 / sizeof(T);
+  constexpr bool WARP = NT == 32;
   using V16 = Vec<T, VEC>;
-  const int64_t row = blockIdx.x / p.splits;
-  const int part = blockIdx.x % p.splits, tid = threadIdx.x;
+  const int splits = WARP ? 1 : p.splits, part = WARP ? 0 : blockIdx.x % splits;
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5) : blockIdx.x / splits;
+  if (WARP && row >= p.rows) return;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
   T* dx = static_cast<T*>(p.dlogits) + row * p.V;
   const int64_t token = p.tokens[row];
@@ -603,7 +673,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd(const __grid_cons
   // the gradient has no stride of its own: its rows may lie on other 16-byte offsets than the logits'
   const bool same = (reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(dx)) % 16 == 0;
   const RowParts<T> parts(x, p.V);
-  const int64_t step = (int64_t)kThreads * p.splits, first = (int64_t)part * kThreads + tid;
+  const int64_t step = (int64_t)NT * splits, first = (int64_t)part * NT + tid;
   const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
   for (int64_t j = first; j < parts.vectors; j += step) {
     float f[VEC];
@@ -621,14 +691,17 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd(const __grid_cons
   const int64_t end_at = first < parts.head ? first : parts.tail0 + (first - parts.head);
   if (first < ends) dx[end_at] = from_f<T>(grad(to_f<T>(x[end_at])));
   // The token's own value and the alternatives', each whole and rounded once, by the CTA that wrote their vector.
-  __syncthreads();
-  for (int i = tid; i <= (p.g_top != nullptr ? p.top : 0); i += kThreads) {
+  if (WARP)
+    __syncwarp();
+  else
+    __syncthreads();
+  for (int i = tid; i <= (p.g_top != nullptr ? p.top : 0); i += NT) {
     const int64_t id = i == 0 ? token : p.top_ids[row * p.top + i - 1];
     if (i == 0 && !use) continue;
     const int64_t owner = id < parts.head ? id
                           : id >= parts.tail0 ? parts.head + id - parts.tail0
                                               : (id - parts.head) / VEC % step;
-    if (owner / kThreads != part) continue;
+    if (owner / NT != part) continue;
     float d = grad(to_f<T>(x[id]));
     if (!none) {
       if (use && id == token) d += gl;
@@ -641,6 +714,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd(const __grid_cons
     dx[id] = from_f<T>(d);
   }
 }
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Short rows leave most of a CTA idle, so a warp takes each, where there are enough of them.
+bool warp_per_row(int64_t rows, int64_t vectors) { return vectors <= 512 && rows >= 2 * num_sms(); }
 
 }  // namespace
 
@@ -659,24 +737,30 @@ void token_logprobs_fwd_launch(const at::Tensor& logits, const at::Tensor& token
   p.V = V;
   p.inv_tau = (float)inv_tau;
   p.c = (float)(inv_tau * 1.4426950408889634);
-  const int64_t vectors = V * logits.element_size() / 16, tiles = std::max<int64_t>(1, (vectors + kTile - 1) / kTile);
-  p.tiles = tiles;
-  // groups small enough for at least 128 in a row, but no more than are looked at in one go
-  while (p.lanes_log < 5 && tiles * kThreads >> p.lanes_log > kColumns) ++p.lanes_log;
+  p.rows = rows;
+  const int64_t vectors = V * logits.element_size() / 16;
+  const bool warp = warp_per_row(rows, vectors);
+  const int64_t threads = warp ? 32 : kThreads, tiles = std::max<int64_t>(1, ceil_div(vectors, threads * kUnroll));
   // Clusters while all CTAs are resident at once (5 on an SM) and each has a tile: 257 x 131072 fp32 45 us with one
   // CTA for a row, 33 us with two, 37 us with four; 4 x 50304 bf16 6.6, 5.5, 4.7 and (eight) 4.2 us.
   int C = 1;
-  while (C < 8 && rows * C * 2 <= 5 * num_sms() && tiles > C) C *= 2;
+  while (!warp && C < 8 && rows * C * 2 <= 5 * num_sms() && tiles > C) C *= 2;
   p.cluster = C;
   MT_CHECK(rows * C < (int64_t(1) << 31), "token_logprobs: too many rows: ", rows);
   at::Tensor maxima;
   if (top > 0) {
-    maxima = at::Tensor(at::detail::empty_cuda({rows, tiles, kThreads >> p.lanes_log}, at::kFloat, logits.device(), c10::nullopt));
+    // groups as large as leave 128 at least in a long row; in a short one single vectors where there are too few others
+    Groups& g = p.groups;
+    g.threads_log = warp ? 5 : 8;
+    while (g.lanes_log < 5 && tiles * threads >> g.lanes_log > kColumns) ++g.lanes_log;
+    g.single = warp && tiles * threads < 3 * top;
+    g.stride = (uint32_t)(g.single ? std::max<int64_t>(1, vectors) : tiles * threads >> g.lanes_log);
+    maxima = at::Tensor(at::detail::empty_cuda({rows, (int64_t)g.stride}, at::kFloat, logits.device(), c10::nullopt));
     p.maxima = maxima.data_ptr<float>();
   }
   auto launch = [&](auto kernel) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(rows * C));
+    cfg.gridDim = dim3((unsigned)(warp ? ceil_div(rows, kThreads / 32) : rows * C));
     cfg.blockDim = dim3(kThreads);
     cfg.stream = cur_stream();
     cudaLaunchAttribute attr{};
@@ -684,24 +768,31 @@ void token_logprobs_fwd_launch(const at::Tensor& logits, const at::Tensor& token
     attr.val.clusterDim.x = (unsigned)C;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = C > 1 ? 1 : 0;
     C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
     MT_LAUNCH_CHECK();
   };
   dispatch_act(logits.scalar_type(), [&](auto t) {
     using T = decltype(t);
-    const bool ent = entropy.defined();
-    if (ent && top > 0)
-      launch(token_logprobs_fwd<T, true, true>);
-    else if (ent)
-      launch(token_logprobs_fwd<T, true, false>);
-    else if (top > 0)
-      launch(token_logprobs_fwd<T, false, true>);
+    auto with = [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      const bool ent = entropy.defined();
+      if (ent && top > 0)
+        launch(token_logprobs_fwd<T, true, true, NT>);
+      else if (ent)
+        launch(token_logprobs_fwd<T, true, false, NT>);
+      else if (top > 0)
+        launch(token_logprobs_fwd<T, false, true, NT>);
+      else
+        launch(token_logprobs_fwd<T, false, false, NT>);
+    };
+    if (warp)
+      with(std::integral_constant<int, 32>{});
     else
-      launch(token_logprobs_fwd<T, false, false>);
+      with(std::integral_constant<int, kThreads>{});
     if (top == 0) return;
     TopParams q{p.logits, p.maxima, p.stats, top_lp.data_ptr<float>(), top_ids.data_ptr<int64_t>(), p.ld, V,
-                tiles, p.inv_tau, (int)top, p.lanes_log};
+                p.inv_tau, (int)top, p.groups};
     token_logprobs_top<T><<<(unsigned)rows, kSelThreads, 0, cur_stream()>>>(q);
     MT_LAUNCH_CHECK();
   });
@@ -732,18 +823,27 @@ void token_logprobs_bwd_launch(const at::Tensor& logits, const at::Tensor& token
   p.V = V;
   p.inv_tau = (float)inv_tau;
   p.c = (float)(inv_tau * 1.4426950408889634);
+  p.rows = rows;
   const int64_t vectors = V * logits.element_size() / 16;
+  const bool warp = warp_per_row(rows, vectors);
   p.splits = 1;
-  while (rows * p.splits < 4 * num_sms() && vectors > (int64_t)kThreads * p.splits) p.splits *= 2;
+  while (!warp && rows * p.splits < 4 * num_sms() && vectors > (int64_t)kThreads * p.splits) p.splits *= 2;
   MT_CHECK(rows * p.splits < (int64_t(1) << 31), "token_logprobs: too many rows: ", rows);
   dispatch_act(logits.scalar_type(), [&](auto t) {
     using T = decltype(t);
-    const unsigned grid = (unsigned)(rows * p.splits);
-    if (g_entropy.defined())
-      token_logprobs_bwd<T, true><<<grid, kThreads, 0, cur_stream()>>>(p);
+    const unsigned grid = (unsigned)(warp ? ceil_div(rows, kThreads / 32) : rows * p.splits);
+    auto with = [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      if (g_entropy.defined())
+        token_logprobs_bwd<T, true, NT><<<grid, kThreads, 0, cur_stream()>>>(p);
+      else
+        token_logprobs_bwd<T, false, NT><<<grid, kThreads, 0, cur_stream()>>>(p);
+      MT_LAUNCH_CHECK();
+    };
+    if (warp)
+      with(std::integral_constant<int, 32>{});
     else
-      token_logprobs_bwd<T, false><<<grid, kThreads, 0, cur_stream()>>>(p);
-    MT_LAUNCH_CHECK();
+      with(std::integral_constant<int, kThreads>{});
   });
 }
 

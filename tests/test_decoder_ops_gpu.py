@@ -590,6 +590,21 @@ def test_logprobs_top(top, rows, V):
     _check_logprobs(x, t, top=top, tau=1.5)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [5, 40, 256, 301, 1003, 2048, 4099])
+def test_logprobs_many_short_rows(dtype, V):
+    """Enough rows for a warp each: every bound on the alternatives, ties, masks, rows off 16-byte offsets."""
+    x, t = _logits(401, V, dtype, 12, 1.0)
+    x[5] = float("-inf")
+    x[6] = 1.0
+    x[7, 3:] = float("-inf")
+    x[8, ::2] = torch.finfo(dtype).min
+    x[9] = torch.finfo(dtype).min
+    t[10] = -1
+    for top in sorted({0, 1, min(7, V), min(20, V), min(64, V)}):
+        _check_logprobs(x, t, top=top, tau=0.8, entropy=top != 7)
+
+
 def test_logprobs_ties_and_order():
     """Rows of one value, of two values, falling, rising, and with all large values in one thread's vectors."""
     V = 40000
