@@ -464,7 +464,7 @@ Shape shape_of(const NormParams& p, int esize) {
   }
   for (const void* q : {p.y, p.n, p.dx, p.dh}) ok = ok && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   if (p.gate_kind == kGateFull) ok = ok && reinterpret_cast<uintptr_t>(p.dgate) % 16 == 0;
-  const int per = (p.d + 255) / 256, groups = per > kMaxWarps ? 2 : 1;
+  const int per = (p.d + 255) / 256, groups = per > kMaxWarps / 2 ? 2 : 1;
   const int threads = (per + groups - 1) / groups * 32;
   ok = ok && ins * groups * threads * 8 * esize <= kSmemBudget;  // a row has to fit into the ring
   return Shape{ok, threads, groups, ins};
@@ -475,10 +475,10 @@ template <typename F>
 void with_shape(const Shape& s, bool all, F&& f) {
   using std::integral_constant;
   auto go = [&](auto al, auto every) {
-    if (s.groups == 2)
+    if (s.groups == 2 && s.threads > 512)
       f(al, integral_constant<int, 2>{}, every, integral_constant<int, 1024>{});
-    else if (s.threads > 512)
-      f(al, integral_constant<int, 1>{}, every, integral_constant<int, 1024>{});
+    else if (s.groups == 2)
+      f(al, integral_constant<int, 2>{}, every, integral_constant<int, 512>{});
     else if (s.threads > 256)
       f(al, integral_constant<int, 1>{}, every, integral_constant<int, 512>{});
     else
