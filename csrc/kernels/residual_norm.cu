@@ -43,25 +43,32 @@ struct NormParams {
   bool want_dpre, want_q;
 };
 
-// Columns of a thread's 8 values in a group of 256 columns: vectors of 16 bytes where rows are aligned
-// (ALIGNED), else single values 32 apart, so that each load of the warp is contiguous.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ int col_of(int group, int lane, int i) {
+// How rows are read and written. kAligned: all start on 16 bytes, so that a thread takes vectors. kShifted: all tensors'
+// rows lie alike, but off 16 bytes; a CTA whose rows are a multiple of 16 / sizeof(T) rows apart sees the same offset in
+// each, takes the vectors that cover its rows, and leaves what lies before and behind them alone. kSingle: anything else,
+// value by value.
+enum Mode : int { kSingle, kAligned, kShifted };
+
+// Place in its row, counted from the first vector's start, of a thread's i-th value in a group of 256: vectors, or single
+// values 32 apart, so that each load of the warp is contiguous.
+template <typename T, int MODE>
+__device__ __forceinline__ int place_of(int group, int lane, int i) {
   constexpr int VEC = 16 / sizeof(T);
-  if constexpr (!ALIGNED) return group * 256 + i * 32 + lane;
+  if constexpr (MODE == kSingle) return group * 256 + i * 32 + lane;
   return group * 256 + (i / VEC) * (32 * VEC) + lane * VEC + i % VEC;
 }
 
 // The rows that a thread has asked for, and their values. The slots of one row lie one input after another, each
 // with one 16-byte vector of every thread after the other. INPUTS: a bit for each input, or 0 where the kernel looks
 // at its parameters for which ones there are.
-template <typename T, bool ALIGNED, int NG, unsigned INPUTS>
+template <typename T, int MODE, int NG, unsigned INPUTS>
 struct Rows {
   static constexpr int VEC = 16 / sizeof(T), NV = 8 / VEC;
   const NormParams& p;
   const unsigned char* mine;  // this thread's first vector in the ring
   uint32_t address;           // the same as a shared-memory address
   int lane, g0, pitch;        // pitch: from a thread's vector to its next
+  int shift;                  // kShifted: values of the first vector that lie before the row
 
   __device__ __forceinline__ Rows(const NormParams& p, const unsigned char* ring)
       : p(p),
@@ -69,7 +76,11 @@ struct Rows {
         address(static_cast<uint32_t>(__cvta_generic_to_shared(mine))),
         lane(threadIdx.x & 31),
         g0((threadIdx.x >> 5) * NG),
-        pitch(blockDim.x * 16) {}
+        pitch(blockDim.x * 16),
+        shift(MODE == kShifted ? (int)((uint64_t)blockIdx.x * p.d % VEC) : 0) {}
+
+  // column of a thread's i-th value; below 0 or from d on: none
+  __device__ __forceinline__ int column(int g, int i) const { return place_of<T, MODE>(g0 + g, lane, i) - shift; }
 
   __device__ __forceinline__ bool has(int t) const { return INPUTS != 0 ? INPUTS >> t & 1 : p.in[t] != nullptr; }
 
@@ -78,19 +89,21 @@ struct Rows {
   }
 
   __device__ __forceinline__ void ask(uint32_t row, int stage) const {
-    if constexpr (ALIGNED) {
+    if constexpr (MODE != kSingle) {
       if (row < p.rows) {
 #pragma unroll
         for (int t = 0; t < kIns; ++t) {
           if (!has(t)) continue;
-          const T* src = row_of(t, row);
+          const T* src = row_of(t, row) - shift;
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-              const int c = col_of<T, true>(g0 + g, lane, k * VEC);
-              copy_async16(address + stage * p.stage + p.slot[t] + (g * NV + k) * pitch, src + (c < p.d ? c : 0),
-                           c < p.d);
+              // what lies behind the row is not read: zeros take its place
+              const int at = place_of<T, MODE>(g0 + g, lane, k * VEC), left = p.d + shift - at;
+              const int bytes = MODE == kAligned ? (left > 0 ? 16 : 0) : max(0, min(16, left * (int)sizeof(T)));
+              copy_async16(address + stage * p.stage + p.slot[t] + (g * NV + k) * pitch, src + (left > 0 ? at : 0),
+                           bytes);
             }
         }
       }
@@ -103,7 +116,7 @@ struct Rows {
     if (!has(input)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = both(0.f);
-    } else if constexpr (ALIGNED) {
+    } else if constexpr (MODE != kSingle) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const uint4 w = *reinterpret_cast<const uint4*>(mine + stage * p.stage + p.slot[input] + (g * NV + k) * pitch);
@@ -117,11 +130,17 @@ struct Rows {
           f[2 * k + 1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
         }
       }
+      if (MODE == kShifted && column(g, 0) < 0) {  // what lies before the row
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (column(g, i) < 0) (i & 1 ? f[i / 2].y : f[i / 2].x) = 0.f;
+        }
+      }
     } else {
       const T* src = row_of(input, row);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int c = col_of<T, false>(g0 + g, lane, i);
+        const int c = column(g, i);
         const float v = c < p.d ? to_f<T>(src[c]) : 0.f;
         if (i & 1)
           f[i / 2].y = v;
@@ -133,10 +152,10 @@ struct Rows {
 
   __device__ __forceinline__ void put(void* out, uint32_t row, int g, const float2 (&f)[4]) const {
     T* dst = static_cast<T*>(out) + (uint64_t)row * (uint32_t)p.d;
-    if constexpr (ALIGNED) {
+    if constexpr (MODE != kSingle) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = col_of<T, true>(g0 + g, lane, k * VEC);
+        const int c = column(g, k * VEC);
         uint4 w;
         if constexpr (sizeof(T) == 2) {
           w = make_uint4(narrow_pair<T>(f[0]), narrow_pair<T>(f[1]), narrow_pair<T>(f[2]), narrow_pair<T>(f[3]));
@@ -144,12 +163,19 @@ struct Rows {
           w = make_uint4(__float_as_uint(f[2 * k].x), __float_as_uint(f[2 * k].y), __float_as_uint(f[2 * k + 1].x),
                          __float_as_uint(f[2 * k + 1].y));
         }
-        if (c < p.d) __stcs(reinterpret_cast<uint4*>(dst + c), w);
+        if (MODE == kAligned ? c < p.d : c >= 0 && c + VEC <= p.d) {
+          __stcs(reinterpret_cast<uint4*>(dst + c), w);
+        } else if (MODE == kShifted) {  // the row's ends
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            if (c + i >= 0 && c + i < p.d) dst[c + i] = reinterpret_cast<const T*>(&w)[i];
+          }
+        }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int c = col_of<T, false>(g0 + g, lane, i);
+        const int c = column(g, i);
         if (c < p.d) dst[c] = from_f<T>(i & 1 ? f[i / 2].y : f[i / 2].x);
       }
     }
@@ -159,9 +185,9 @@ struct Rows {
   __device__ __forceinline__ void weight(const float* w, int g, float none, float2 (&f)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c0 = col_of<T, ALIGNED>(g0 + g, lane, 2 * i), c1 = col_of<T, ALIGNED>(g0 + g, lane, 2 * i + 1);
-      f[i].x = w != nullptr && c0 < p.d ? w[c0] : none;
-      f[i].y = w != nullptr && c1 < p.d ? w[c1] : none;
+      const int c0 = column(g, 2 * i), c1 = column(g, 2 * i + 1);
+      f[i].x = w != nullptr && c0 >= 0 && c0 < p.d ? w[c0] : none;
+      f[i].y = w != nullptr && c1 >= 0 && c1 < p.d ? w[c1] : none;
     }
   }
 
@@ -218,11 +244,11 @@ __device__ __forceinline__ float3 cta_sum3(float3 v, float4* red, int& par) {
 
 // ALL: there are a branch and a pre norm, and no gate per element -- what a training step calls; with this known, and
 // the rest done by arithmetic (no post norm is rh = 1), a row takes two thirds of the instructions.
-template <typename T, bool ALIGNED, int NG, bool ALL, int MAXT, int MINB>
+template <typename T, int MODE, int NG, bool ALL, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[2 * kMaxWarps];
-  const Rows<T, ALIGNED, NG, ALL ? 1u << kX | 1u << kH : 0u> in(p, ring);
+  const Rows<T, MODE, NG, ALL ? 1u << kX | 1u << kH : 0u> in(p, ring);
   const float inv_d = 1.f / p.d;
   const bool branch = in.has(kH);
   int par = 0, stage = 0;
@@ -244,7 +270,7 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
       gate = __shfl_sync(0xffffffffu, gates, turn);
       turn = (turn + 1) & 31;
     }
-    if constexpr (ALIGNED) copy_async_wait(p.depth - 1);
+    if constexpr (MODE != kSingle) copy_async_wait(p.depth - 1);
     float2 y[NG][4];
     if (branch) {
       float rh = 1.f;
@@ -297,16 +323,16 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
     }
     stage = stage + 1 == p.depth ? 0 : stage + 1;
   }
-  if constexpr (ALIGNED) copy_async_wait(0);
+  if constexpr (MODE != kSingle) copy_async_wait(0);
 }
 
 // part: [gridDim.x][2][d], the CTA's sums of dn yh (dpre) and of r Y hh (q; with the gate of each element)
 // ALL: as in the forward, and both gradients come in and both are wanted.
-template <typename T, bool ALIGNED, int NG, bool ALL, int MAXT, int MINB>
+template <typename T, int MODE, int NG, bool ALL, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float4 red[2 * kMaxWarps];
-  const Rows<T, ALIGNED, NG, ALL ? 1u << kX | 1u << kH | 1u << kDy | 1u << kDn : 0u> in(p, ring);
+  const Rows<T, MODE, NG, ALL ? 1u << kX | 1u << kH | 1u << kDy | 1u << kDn : 0u> in(p, ring);
   const float inv_d = 1.f / p.d;
   const bool branch = in.has(kH), full = !ALL && p.gate_kind == kGateFull, post = p.post != nullptr;
   int par = 0, stage = 0;
@@ -337,7 +363,7 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
     const float rh = __shfl_sync(kAll, rhs, turn), ry = __shfl_sync(kAll, rys, turn),
                 gate = __shfl_sync(kAll, gates, turn);
     turn = (turn + 1) & 31;
-    if constexpr (ALIGNED) copy_async_wait(p.depth - 1);
+    if constexpr (MODE != kSingle) copy_async_wait(p.depth - 1);
     float2 hh[NG][4], yh[NG][4], t[NG][4];  // t = dy + ry u, so that Y = t - ry yh mean(u yh)
     // sums of u yh, and of c = e hh with t and yh
     float2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f);
@@ -406,15 +432,15 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
     }
     stage = stage + 1 == p.depth ? 0 : stage + 1;
   }
-  if constexpr (ALIGNED) copy_async_wait(0);
+  if constexpr (MODE != kSingle) copy_async_wait(0);
   if (p.part == nullptr) return;
   float* part = p.part + (int64_t)blockIdx.x * 2 * p.d;
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = col_of<T, ALIGNED>(in.g0 + g, in.lane, i);
-      if (c >= p.d) continue;
+      const int c = in.column(g, i);
+      if (c < 0 || c >= p.d) continue;
       if (p.want_dpre) part[c] = i & 1 ? sum_pre[g][i / 2].y : sum_pre[g][i / 2].x;
       if (p.want_q) part[p.d + c] = i & 1 ? sum_q[g][i / 2].y : sum_q[g][i / 2].x;
     }
@@ -449,53 +475,68 @@ __global__ void __launch_bounds__(kFinishWarps * 32)
 }
 
 struct Shape {
-  bool aligned;
+  Mode mode;
   int threads, groups, ins;
 };
 
-// Rows are read in 16-byte vectors where every tensor's rows start on 16 bytes.
 Shape shape_of(const NormParams& p, int esize) {
   const int v = 16 / esize;
-  bool ok = p.d % v == 0;
+  bool ok = true;
   int ins = 0;
   for (int t = 0; t < kIns; ++t) {
-    ok = ok && p.ld[t] % v == 0 && reinterpret_cast<uintptr_t>(p.in[t]) % 16 == 0;
-    ins += p.in[t] != nullptr;
+    if (p.in[t] == nullptr) continue;
+    ok = ok && reinterpret_cast<uintptr_t>(p.in[t]) % 16 == 0 && (p.rows == 1 || (p.ld[t] + v - p.d % v) % v == 0);
+    ++ins;
   }
   for (const void* q : {p.y, p.n, p.dx, p.dh}) ok = ok && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   if (p.gate_kind == kGateFull) ok = ok && reinterpret_cast<uintptr_t>(p.dgate) % 16 == 0;
-  const int per = (p.d + 255) / 256, groups = per > kMaxWarps / 2 ? 2 : 1;
-  const int threads = (per + groups - 1) / groups * 32;
-  ok = ok && ins * groups * threads * 8 * esize <= kSmemBudget;  // a row has to fit into the ring
-  return Shape{ok, threads, groups, ins};
+  Shape s{!ok ? kSingle : p.d % v == 0 ? kAligned : kShifted, 0, 0, ins};
+  const int per = (p.d + (s.mode == kShifted ? v - 1 : 0) + 255) / 256;
+  s.groups = per > kMaxWarps / 2 ? 2 : 1;
+  s.threads = (per + s.groups - 1) / s.groups * 32;
+  // a row has to fit into the ring, and into a CTA
+  if (s.mode != kSingle && (ins * s.groups * s.threads * 8 * esize > kSmemBudget || s.threads > 1024)) {
+    s.mode = kSingle;
+    s.threads = std::min(s.threads, 1024);
+  }
+  return s;
 }
 
-// f(ALIGNED, NG, ALL, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
+// f(MODE, NG, ALL, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
 template <typename F>
 void with_shape(const Shape& s, bool all, F&& f) {
   using std::integral_constant;
-  auto go = [&](auto al, auto every) {
+  auto go = [&](auto mode, auto every) {
     if (s.groups == 2 && s.threads > 512)
-      f(al, integral_constant<int, 2>{}, every, integral_constant<int, 1024>{});
+      f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 1024>{});
     else if (s.groups == 2)
-      f(al, integral_constant<int, 2>{}, every, integral_constant<int, 512>{});
+      f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 512>{});
     else if (s.threads > 256)
-      f(al, integral_constant<int, 1>{}, every, integral_constant<int, 512>{});
+      f(mode, integral_constant<int, 1>{}, every, integral_constant<int, 512>{});
     else
-      f(al, integral_constant<int, 1>{}, every, integral_constant<int, 256>{});
+      f(mode, integral_constant<int, 1>{}, every, integral_constant<int, 256>{});
   };
-  if (s.aligned && all)
-    go(std::true_type{}, std::true_type{});
-  else if (s.aligned)
-    go(std::true_type{}, std::false_type{});
+  auto with = [&](auto mode) { all ? go(mode, std::true_type{}) : go(mode, std::false_type{}); };
+  if (s.mode == kAligned)
+    with(integral_constant<int, kAligned>{});
+  else if (s.mode == kShifted)
+    with(integral_constant<int, kShifted>{});
   else
-    go(std::false_type{}, std::false_type{});
+    go(integral_constant<int, kSingle>{}, std::false_type{});
+}
+
+// The grid, with rows of a CTA that lie alike where that is needed.
+unsigned grid_of(int64_t wanted, const NormParams& p, const Shape& s, int esize) {
+  int64_t grid = std::min<int64_t>(p.rows, wanted);
+  const int v = 16 / esize;
+  if (s.mode == kShifted && grid < p.rows) grid = std::min<int64_t>(p.rows, std::max<int64_t>(v, grid / v * v));
+  return (unsigned)grid;
 }
 
 // The ring's depth for `fit` CTAs per SM, and the CTAs that are resident with it.
 int64_t plan_ring(NormParams& p, const Shape& s, int esize, int fit, int deepest) {
   p.depth = 1;
-  if (s.aligned) {
+  if (s.mode != kSingle) {
     for (int t = 0, at = 0; t < kIns; ++t) {
       p.slot[t] = at;
       at += p.in[t] != nullptr ? s.groups * s.threads * 8 * esize : 0;
@@ -560,11 +601,11 @@ void residual_norm_fwd_launch(const ResidualNormArgs& a, const at::Tensor& y, co
     using T = decltype(t);
     const Shape s = shape_of(p, sizeof(T));
     const bool all = p.in[kH] != nullptr && p.n != nullptr && a.gate_kind != kGateFull;
-    with_shape(s, all, [&](auto al, auto ng, auto every, auto maxt) {
+    with_shape(s, all, [&](auto mode, auto ng, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 1024 ? 1 : 1024 / kMaxT;
       const int fit = std::min(16, kMinB * kMaxT / s.threads);
-      const unsigned grid = (unsigned)std::min<int64_t>(p.rows, plan_ring(p, s, sizeof(T), fit, 4));
-      launch_norm(residual_norm_fwd<T, decltype(al)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, grid);
+      const unsigned grid = grid_of(plan_ring(p, s, sizeof(T), fit, 4), p, s, sizeof(T));
+      launch_norm(residual_norm_fwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, grid);
     });
   });
 }
@@ -597,18 +638,19 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
     const Shape s = shape_of(p, sizeof(T));
     bool all = a.gate_kind != kGateFull;
     for (const void* q : {p.in[kH], p.in[kDy], p.in[kDn], (const void*)p.dx, (const void*)p.dh}) all = all && q != nullptr;
-    with_shape(s, all, [&](auto al, auto ng, auto every, auto maxt) {
+    with_shape(s, all, [&](auto mode, auto ng, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 256 ? 2 : 1;
       const int fit = std::min(16, kMinB * kMaxT / s.threads);
-      int64_t grid = std::min<int64_t>(p.rows, plan_ring(p, s, sizeof(T), fit, 4));
+      int64_t grid = plan_ring(p, s, sizeof(T), fit, 4);
+      // a few rows for each CTA at least: its partial sums cost as much as two rows
+      if (p.want_dpre || p.want_q) grid = std::min<int64_t>(grid, (p.rows + 3) / 4);
+      grid = grid_of(grid, p, s, sizeof(T));
       at::Tensor part;
       if (p.want_dpre || p.want_q) {
-        // a few rows for each CTA at least: its partial sums cost as much as two rows
-        grid = std::min<int64_t>(grid, (p.rows + 3) / 4);
         part = at::Tensor(at::detail::empty_cuda({grid, 2, (int64_t)p.d}, at::kFloat, a.x.device(), c10::nullopt));
         p.part = part.data_ptr<float>();
       }
-      launch_norm(residual_norm_bwd<T, decltype(al)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, (unsigned)grid);
+      launch_norm(residual_norm_bwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, (unsigned)grid);
       if (p.part != nullptr) {
         residual_norm_finish<<<dim3((p.d + 31) / 32, p.want_dpre + p.want_q), kFinishWarps * 32, 0, cur_stream()>>>(
             p.part, (int)grid, p.d, p.want_dpre, p.alpha, a.gate_kind == kGateChannel ? p.gate : nullptr, p.post,

@@ -102,9 +102,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 
-// 16-byte asynchronous copy global -> shared (address d); nothing is read and zeros are written where `there` is false.
-__device__ __forceinline__ void copy_async16(uint32_t d, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(there ? 16 : 0) : "memory");
+// 16-byte asynchronous copy global -> shared (address d); reads the first `bytes` bytes only, zeros take the others' place.
+__device__ __forceinline__ void copy_async16(uint32_t d, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most `pending` (0 .. 3) of this thread's youngest groups are in flight.

@@ -388,6 +388,28 @@ def test_residual_norm_many_rows():
     _check_norm(t, dy, dn)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,d", [(7, 77), (9, 77), (2011, 77), (601, 1003), (333, 2047), (5, 8191), (1200, 4097),
+                                    (2, 9), (300, 9), (37, 260)])
+@pytest.mark.parametrize("gate", ["channel", "full"])
+def test_residual_norm_rows_off_16_bytes(dtype, rows, d, gate):
+    t, dy, dn = _norm_case(rows, d, dtype, True, True, gate, 14)
+    _check_norm(t, dy, dn)
+
+
+def test_residual_norm_rows_off_16_bytes_of_a_wider_matrix():
+    """Rows of 257 values, 769 apart: what lies between them is neither used nor, in the outputs, written."""
+    g = _gen(15)
+    wide = torch.full((40, 769), float("nan"), device=DEV, dtype=BF)
+    t, dy, dn = _norm_case(40, 257, BF, True, True, "channel", 15)
+    for at in (0, 512):
+        x = wide.clone()
+        x[:, at:at + 257] = torch.randn(40, 257, generator=g, device=DEV).to(BF)
+        _check_norm(dict(t, x=x[:, at:at + 257]), dy, dn)
+        _check_norm(dict(t, h=x[:, at:at + 257]), dy, dn)
+        _check_norm(t, x[:, at:at + 257], dn)
+
+
 def test_residual_norm_zero_gate_and_zero_rows():
     t, dy, dn = _norm_case(6, 320, F32, True, True, "row", 5)
     t["gate"][1] = 0.0
