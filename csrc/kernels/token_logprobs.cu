@@ -30,8 +30,8 @@ namespace {
 
 constexpr int kThreads = 256;  // of a CTA of the first pass and of the backward
 constexpr int kUnroll = 4;     // vectors of a thread in flight
-constexpr int kSelThreads = 128;
-constexpr int kColumns = 2 * kSelThreads;
+constexpr int kTopThreads = 128;  // of a CTA that picks the alternatives of a row
+constexpr int kColumns = 256;
 constexpr int kManyWinners = 128;
 constexpr int kMaxTop = 64;
 constexpr int kHits = 512, kCandidates = 768;
@@ -223,8 +223,8 @@ __device__ __forceinline__ Running shuffle_join(Running a, float c) {
 template <typename T>
 struct RowParts {
   static constexpr int VEC = 16 / sizeof(T);
-  int64_t head, vectors, tail0;
-  __device__ __forceinline__ RowParts(const T* row, int64_t V) {
+  int64_t head, vectors, tail0, end;
+  __device__ __forceinline__ RowParts(const T* row, int64_t V) : end(V) {
     const int64_t off = (16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T);
     head = off < V ? off : V;
     vectors = (V - head) / VEC;
@@ -260,9 +260,276 @@ struct FwdParams {
   Groups groups;
 };
 
-// NT: threads that share a row, a CTA (or one of a cluster) or a warp.
-template <typename T, bool ENT, bool TOP, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : 5) token_logprobs_fwd(const __grid_constant__ FwdParams p) {
+struct TopParams {
+  const float* maxima;  // as the first kernel's
+  float* top_lp;
+  int64_t* top_ids;
+  float inv_tau;
+  int top;
+  Groups groups;
+};
+
+struct TopShared {
+  int4 group[kColumns / 4];  // maxima of columns, or of a few together
+  uint4 hit[kHits];             // vectors with a value from the bound on
+  int hit_at[kHits];
+  long long cand[kCandidates];
+  int winners[kColumns];
+  int n_hit, n_cand, n_won, floor, larger;
+  long long threshold, red[kThreads / 32];
+};
+
+// Appends `column` to the winners where `win`.
+__device__ __forceinline__ void push_winner(TopShared& ts, bool win, int column) {
+  const unsigned all = __ballot_sync(0xffffffffu, win), lane = threadIdx.x & 31;
+  int base = 0;
+  if (lane == 0 && all != 0) base = atomicAdd(&ts.n_won, __popc(all));
+  const int at = __shfl_sync(0xffffffffu, base, 0) + __popc(all & ((1u << lane) - 1));
+  if (win) ts.winners[at] = column;
+}
+
+// The alternatives of a row, by a CTA of NT threads; m and l2s as in the statistics. The groups c, c + kColumns, ... of
+// the row are its column c; a thread looks after columns tid, tid + NT, ...
+template <typename T, int NT>
+__device__ __forceinline__ void pick_top(const TopParams& p, const T* x, const RowParts<T>& parts, int64_t row, float m,
+                                         float l2s, TopShared& ts) {
+  constexpr int VEC = 16 / sizeof(T), PER = kColumns / NT;
+  constexpr unsigned kAll = 0xffffffffu;
+  using V16 = Vec<T, VEC>;
+  const int tid = threadIdx.x;
+  const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
+  static_assert(kUnroll == 4, "the shifts here");
+  const int log = p.groups.lanes_log, threads_log = p.groups.threads_log;
+  const bool single = p.groups.single;
+  const unsigned vectors = (unsigned)parts.vectors;
+  const unsigned full = vectors >> (threads_log + 2), rest = vectors - (full << (threads_log + 2));  // tiles, vectors
+  const unsigned groups = single ? vectors : (full + (rest != 0)) << (threads_log - log);
+  // groups with values, and the columns that hold them
+  const unsigned real = single ? vectors
+                               : (full << (threads_log - log)) + ((min(rest, 1u << threads_log) + (1u << log) - 1) >> log);
+  const int columns = (int)min(real, (unsigned)kColumns);
+  int value[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) value[i] = INT_MIN;
+  for (unsigned g = tid; g < groups; g += kColumns) {
+    const float* most = p.maxima + row * p.groups.stride + g;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (g + i * NT < groups) value[i] = max(value[i], order_of(most[i * NT]));
+    }
+  }
+  int column_log = single ? 0 : 2 + log;  // vectors of a column
+  const int group_log = column_log;
+  while ((unsigned)kColumns << (column_log - group_log) < groups) ++column_log;
+  // the r-th vector of a column, in the order of the row; `vectors` or more for none
+  auto vector_of = [&](unsigned column, unsigned r) {
+    if (single) return column + r * kColumns;
+    const unsigned round = r >> log, g = column + (round >> 2) * kColumns, tile = g >> (threads_log - log);
+    return (tile << (threads_log + 2)) + ((round & 3) << threads_log) +
+           ((g << log) & ((1u << threads_log) - 1)) + (r & ((1u << log) - 1));
+  };
+  if (tid == 0) {
+    ts.n_hit = ts.n_cand = ts.n_won = ts.larger = 0;
+    ts.floor = INT_MAX;
+    ts.threshold = kNoKey;  // stays where fewer equal values are left than needed
+  }
+
+  // The bound: the k-th largest of the columns' maxima, or, where there are many more columns than that, of the maxima of
+  // 2 or 4 columns: fewer comparisons, shared by the threads that hold these columns, for a few more values to rank.
+  const int merged = columns >= 6 * p.top ? 4 : columns >= 3 * p.top ? 2 : 1;
+  int low = INT_MAX;  // smallest maximum that fewer than k others exceed
+  int* list = reinterpret_cast<int*>(ts.group);
+  if (merged < PER || (PER == 1 && merged == 1)) {
+    int above[PER] = {};
+#pragma unroll
+    for (int k = 0; k < PER; ++k) list[tid + k * NT] = value[k];
+    __syncthreads();
+#pragma unroll 4
+    for (int i = 0; i < kColumns / 4; ++i) {
+      const int4 q = ts.group[i];
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        above[k] += (q.x > value[k]) + (q.y > value[k]) + (q.z > value[k]) + (q.w > value[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (value[k] != INT_MIN && above[k] < p.top) low = min(low, value[k]);
+    }
+  } else {
+    const int share = merged / PER;  // threads of a maximum: 1, 2 or 4
+    int best = value[0], above = 0;
+#pragma unroll
+    for (int k = 1; k < PER; ++k) best = max(best, value[k]);
+    for (int o = 1; o < share; o *= 2) best = max(best, __shfl_xor_sync(kAll, best, o));
+    if (tid % share == 0) list[tid / share] = best;
+    __syncthreads();
+    const int n = NT / share / share / 4;
+    const int4* o = ts.group + tid % share * n;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const int4 q = o[i];
+      above += (q.x > best) + (q.y > best) + (q.z > best) + (q.w > best);
+    }
+    for (int o = 1; o < share; o *= 2) above += __shfl_xor_sync(kAll, above, o);
+    if (best != INT_MIN && above < p.top) low = best;
+  }
+  low = __reduce_min_sync(kAll, low);
+  if ((tid & 31) == 0) atomicMin(&ts.floor, low);
+  __syncthreads();
+  // with fewer columns than alternatives every value counts
+  const int floor = columns < p.top ? INT_MIN + 1 : ts.floor;
+  long long threshold = columns < p.top ? kNoKey : (long long)floor * 0x100000000ll;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) push_winner(ts, value[i] >= floor, tid + i * NT);
+  __syncthreads();
+  int won = ts.n_won;
+  if (won > kManyWinners) {
+    // Many columns share the bound (equal or masked logits): of these, those with the lowest indexes win.
+    long long k[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int column = tid + i * NT;
+      k[i] = kNoKey;
+      if (value[i] == floor) {
+        for (unsigned q = 0; q >> column_log == 0 && k[i] == kNoKey; ++q) {
+          const unsigned j = vector_of(column, q);
+          if (j >= vectors) continue;
+          const V16 v = xv[j];
+#pragma unroll
+          for (int e = VEC - 1; e >= 0; --e) {
+            const float f = to_f<T>(v.v[e]);
+            if (order_of(f) == floor) k[i] = key_of(f, parts.head + (int64_t)j * VEC + e);
+          }
+        }
+      }
+      ts.cand[column] = k[i];
+      const unsigned more = __ballot_sync(kAll, value[i] > floor);
+      if ((tid & 31) == 0) atomicAdd(&ts.larger, __popc(more));
+    }
+    __syncthreads();
+    if (tid == 0) ts.n_won = 0;
+    const int need = p.top - ts.larger;  // so many of the equal ones
+    int r[PER] = {};
+    for (int i = 0; i < kColumns; ++i) {
+#pragma unroll
+      for (int n = 0; n < PER; ++n) r[n] += ts.cand[i] > k[n];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      push_winner(ts, value[i] > floor || (k[i] != kNoKey && r[i] < need), tid + i * NT);
+      if (k[i] != kNoKey && r[i] == need - 1) ts.threshold = k[i];
+    }
+    __syncthreads();
+    won = ts.n_won;
+    threshold = need > 0 ? ts.threshold : (long long)(floor + 1) * 0x100000000ll;
+  }
+
+  const float floor_value = threshold == kNoKey ? -INFINITY : key_value(threshold);
+  auto offer = [&](float f, int64_t index) {
+    if (f < floor_value) return;
+    const long long k = key_of(f, index);
+    if (k < threshold) return;
+    const int at = atomicAdd(&ts.n_cand, 1);
+    if (at < kCandidates) ts.cand[at] = k;
+  };
+  const int64_t last_equal = key_index(threshold);  // values that equal the bound count up to here
+  const unsigned todo = (unsigned)won << column_log;
+  for (unsigned i = tid; i < todo; i += kUnroll * NT) {
+    V16 v[kUnroll];
+    unsigned at[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const unsigned q = i + u * NT;
+      at[u] = q < todo ? vector_of(ts.winners[q >> column_log], q & ((1u << column_log) - 1)) : vectors;
+      if (at[u] < vectors) v[u] = xv[at[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (at[u] >= vectors) continue;
+      const V16 one[1] = {v[u]};
+      const float vm = largest<T>(one);
+      if (vm < floor_value || (vm == floor_value && parts.head + (int64_t)at[u] * VEC > last_equal)) continue;
+      const int h = atomicAdd(&ts.n_hit, 1);
+      if (h >= kHits) continue;
+      ts.hit[h] = *reinterpret_cast<const uint4*>(&v[u]);
+      ts.hit_at[h] = (int)at[u];
+    }
+  }
+  __syncthreads();
+  const int hits = ts.n_hit;
+  for (int i = tid; i < min(hits, kHits) * VEC; i += NT)
+    offer(to_f<T>(reinterpret_cast<const T*>(ts.hit)[i]), parts.head + (int64_t)ts.hit_at[i / VEC] * VEC + i % VEC);
+  // the row's ends, at most 2 (VEC - 1) values
+  const int64_t end_at = tid < parts.head ? tid : parts.tail0 + (tid - parts.head);
+  const bool end = tid < parts.head + (parts.end - parts.tail0);
+  if (end) offer(to_f<T>(x[end_at]), end_at);
+  __syncthreads();
+
+  auto put = [&](int i, long long k) {
+    p.top_ids[row * p.top + i] = key_index(k);
+    p.top_lp[row * p.top + i] = l2s == -INFINITY ? -INFINITY : (key_value(k) - m) * p.inv_tau - l2s * kLn2;
+  };
+  const int n = ts.n_cand;
+  if (hits <= kHits && n <= kCandidates) {
+    // each candidate's place is the number of larger ones, which 4 threads count
+    const int part = tid & 3;
+    for (int i0 = 0; i0 < n; i0 += NT / 4) {
+      const int i = i0 + (tid >> 2);
+      const long long k = i < n ? ts.cand[i] : kNoKey;
+      int r = 0;
+#pragma unroll 4
+      for (int j = part; j < n; j += 4) r += ts.cand[j] > k;
+      r += __shfl_xor_sync(kAll, r, 1);
+      r += __shfl_xor_sync(kAll, r, 2);
+      if (part == 0 && i < n && r < p.top) put(r, k);
+    }
+    return;
+  }
+  // More values above the bound than there is room for: rows whose largest values all lie in a few columns. Takes the
+  // largest key below the last one, k times over.
+  long long last = LLONG_MAX;
+  for (int i = 0; i < p.top; ++i) {
+    long long k = kNoKey;
+    for (int64_t j = tid; j < parts.vectors; j += NT) {
+      const V16 v = xv[j];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const long long q = key_of(to_f<T>(v.v[e]), parts.head + j * VEC + e);
+        if (q < last) k = max(k, q);
+      }
+    }
+    if (end) {
+      const long long q = key_of(to_f<T>(x[end_at]), end_at);
+      if (q < last) k = max(k, q);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(kAll, k, o));
+    __syncthreads();
+    if ((tid & 31) == 0) ts.red[tid >> 5] = k;
+    __syncthreads();
+    for (int w = 0; w < NT / 32; ++w) k = max(k, ts.red[w]);
+    if (tid == 0) put(i, k);
+    last = k;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTopThreads)
+    token_logprobs_top(const __grid_constant__ TopParams p, const T* logits, int64_t ld, int64_t V, const float* stats) {
+  __shared__ TopShared ts;
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * ld;
+  pick_top<T, kTopThreads>(p, x, RowParts<T>(x, V), row, stats[2 * row], stats[2 * row + 1], ts);
+}
+
+enum Top : int { kNoTop, kTopMaxima, kTopHere };
+
+// NT: threads that share a row, a CTA (or one of a cluster) or a warp. TOP: the maxima for the alternatives are written,
+// or the alternatives picked at once, by the row's first CTA.
+template <typename T, bool ENT, int TOP, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : TOP == kTopHere ? 2 : 5)
+    token_logprobs_fwd(const __grid_constant__ FwdParams p, const __grid_constant__ TopParams top) {
   constexpr int VEC = 16 / sizeof(T), TILE = NT * kUnroll;
   constexpr bool WARP = NT == 32;
   using V16 = Vec<T, VEC>;
@@ -316,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : 5) token_logprobs_fwd
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) v[u] = from[u * NT];
     const float vm = take(v);
-    if constexpr (TOP) keep(v, tile, vm);
+    if constexpr (TOP != kNoTop) keep(v, tile, vm);
   }
   if (tile < tiles) {  // the last one, where it is not full
     const int64_t j = tile * TILE + tid;
@@ -329,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : 5) token_logprobs_fwd
       const V16 one[1] = {v[u]};
       if (tile * TILE + u * NT < parts.vectors) vm = fmaxf(vm, take(one));
     }
-    if constexpr (TOP) keep(v, tile, vm);
+    if constexpr (TOP != kNoTop) keep(v, tile, vm);
   }
   Running a;
   if (!fast_done<T, ENT>(sums, p.c, a)) {
@@ -366,269 +633,24 @@ __global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : 5) token_logprobs_fwd
       cluster.sync();  // the others' shared memory lives until it has been read
     }
   }
-  if (rank != 0 || tid != 0) return;
-  // a row without any possible token has S = 0
-  const bool none = a.s == 0.f;
-  const float l2s = none ? -INFINITY : log2f(a.s);
-  float lp = 0.f;
-  if (token >= 0 && token < p.V) lp = none ? -INFINITY : (token_value - a.m) * p.inv_tau - l2s * kLn2;
-  p.logprob[row] = lp;
-  p.stats[2 * row] = a.m;
-  p.stats[2 * row + 1] = l2s;
-  if (ENT) p.entropy[row] = none ? 0.f : (l2s - a.w / a.s) * kLn2;
-}
-
-struct TopParams {
-  const void* logits;
-  const float* maxima;
-  const float* stats;
-  float* top_lp;
-  int64_t* top_ids;
-  int64_t ld, V;
-  float inv_tau;
-  int top;
-  Groups groups;
-};
-
-struct TopShared {
-  int4 group[kColumns / 4];  // maxima of columns, or of a few together
-  uint4 hit[kHits];             // vectors with a value from the bound on
-  int hit_at[kHits];
-  long long cand[kCandidates];
-  int winners[kColumns];
-  int n_hit, n_cand, n_won, floor, larger;
-  long long threshold, red[kSelThreads / 32];
-};
-
-// Appends `column` to the winners where `win`.
-__device__ __forceinline__ void push_winner(TopShared& ts, bool win, int column) {
-  const unsigned all = __ballot_sync(0xffffffffu, win), lane = threadIdx.x & 31;
-  int base = 0;
-  if (lane == 0 && all != 0) base = atomicAdd(&ts.n_won, __popc(all));
-  const int at = __shfl_sync(0xffffffffu, base, 0) + __popc(all & ((1u << lane) - 1));
-  if (win) ts.winners[at] = column;
-}
-
-// One CTA per row. The groups c, c + kColumns, ... of the row are its column c; a thread looks after columns tid and
-// tid + kSelThreads.
-template <typename T>
-__global__ void __launch_bounds__(kSelThreads) token_logprobs_top(const __grid_constant__ TopParams p) {
-  constexpr int VEC = 16 / sizeof(T);
-  constexpr unsigned kAll = 0xffffffffu;
-  using V16 = Vec<T, VEC>;
-  __shared__ TopShared ts;
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-  const RowParts<T> parts(x, p.V);
-  const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
-  static_assert(kUnroll == 4, "the shifts here");
-  const int log = p.groups.lanes_log, threads_log = p.groups.threads_log;
-  const bool single = p.groups.single;
-  const unsigned vectors = (unsigned)parts.vectors;
-  const unsigned full = vectors >> (threads_log + 2), rest = vectors - (full << (threads_log + 2));  // tiles, vectors
-  const unsigned groups = single ? vectors : (full + (rest != 0)) << (threads_log - log);
-  // groups with values, and the columns that hold them
-  const unsigned real = single ? vectors
-                               : (full << (threads_log - log)) + ((min(rest, 1u << threads_log) + (1u << log) - 1) >> log);
-  const int columns = (int)min(real, (unsigned)kColumns);
-  int value[2] = {INT_MIN, INT_MIN};
-  for (unsigned g = tid; g < groups; g += kColumns) {
-    const float* most = p.maxima + row * p.groups.stride + g;
-    value[0] = max(value[0], order_of(most[0]));
-    if (g + kSelThreads < groups) value[1] = max(value[1], order_of(most[kSelThreads]));
-  }
-  int column_log = single ? 0 : 2 + log;  // vectors of a column
-  const int group_log = column_log;
-  while ((unsigned)kColumns << (column_log - group_log) < groups) ++column_log;
-  // the r-th vector of a column, in the order of the row; `vectors` or more for none
-  auto vector_of = [&](unsigned column, unsigned r) {
-    if (single) return column + r * kColumns;
-    const unsigned round = r >> log, g = column + (round >> 2) * kColumns, tile = g >> (threads_log - log);
-    return (tile << (threads_log + 2)) + ((round & 3) << threads_log) +
-           ((g << log) & ((1u << threads_log) - 1)) + (r & ((1u << log) - 1));
-  };
-  const float m = p.stats[2 * row], l2s = p.stats[2 * row + 1];
+  if (rank != 0) return;
   if (tid == 0) {
-    ts.n_hit = ts.n_cand = ts.n_won = ts.larger = 0;
-    ts.floor = INT_MAX;
-    ts.threshold = kNoKey;  // stays where fewer equal values are left than needed
+    // a row without any possible token has S = 0
+    const bool none = a.s == 0.f;
+    const float l2s = none ? -INFINITY : log2f(a.s);
+    float lp = 0.f;
+    if (token >= 0 && token < p.V) lp = none ? -INFINITY : (token_value - a.m) * p.inv_tau - l2s * kLn2;
+    p.logprob[row] = lp;
+    p.stats[2 * row] = a.m;
+    p.stats[2 * row + 1] = l2s;
+    if (ENT) p.entropy[row] = none ? 0.f : (l2s - a.w / a.s) * kLn2;
+    all.m = a.m;
+    all.s = l2s;
   }
-
-  // The bound: the k-th largest of the columns' maxima, or, where there are many more columns than that, of the maxima of
-  // 2 or 4 columns: fewer comparisons, shared by two threads for 4 columns, for a few more values to rank.
-  const int merged = columns >= 6 * p.top ? 4 : columns >= 3 * p.top ? 2 : 1;
-  int low = INT_MAX;  // smallest maximum that fewer than k others exceed
-  if (merged == 1) {
-    int* list = reinterpret_cast<int*>(ts.group);
-    list[tid] = value[0];
-    list[tid + kSelThreads] = value[1];
+  if constexpr (TOP == kTopHere) {
+    __shared__ TopShared ts;
     __syncthreads();
-    int above[2] = {0, 0};
-#pragma unroll 4
-    for (int i = 0; i < kColumns / 4; ++i) {
-      const int4 q = ts.group[i];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        above[k] += (q.x > value[k]) + (q.y > value[k]) + (q.z > value[k]) + (q.w > value[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (value[k] != INT_MIN && above[k] < p.top) low = min(low, value[k]);
-    }
-  } else {
-    const bool four = merged == 4;
-    int best = max(value[0], value[1]), above = 0;
-    if (four) best = max(best, __shfl_xor_sync(kAll, best, 1));
-    if (!four || (tid & 1) == 0) reinterpret_cast<int*>(ts.group)[four ? tid >> 1 : tid] = best;
-    __syncthreads();
-    const int n = four ? kSelThreads / 16 : kSelThreads / 4;
-    const int4* o = ts.group + (four ? (tid & 1) * n : 0);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const int4 q = o[i];
-      above += (q.x > best) + (q.y > best) + (q.z > best) + (q.w > best);
-    }
-    if (four) above += __shfl_xor_sync(kAll, above, 1);
-    if (best != INT_MIN && above < p.top) low = best;
-  }
-  low = __reduce_min_sync(kAll, low);
-  if ((tid & 31) == 0) atomicMin(&ts.floor, low);
-  __syncthreads();
-  // with fewer columns than alternatives every value counts
-  const int floor = columns < p.top ? INT_MIN + 1 : ts.floor;
-  long long threshold = columns < p.top ? kNoKey : (long long)floor * 0x100000000ll;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) push_winner(ts, value[i] >= floor, tid + i * kSelThreads);
-  __syncthreads();
-  int won = ts.n_won;
-  if (won > kManyWinners) {
-    // Many columns share the bound (equal or masked logits): of these, those with the lowest indexes win.
-    long long k[2] = {kNoKey, kNoKey};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int column = tid + i * kSelThreads;
-      if (value[i] == floor) {
-        for (unsigned q = 0; q >> column_log == 0 && k[i] == kNoKey; ++q) {
-          const unsigned j = vector_of(column, q);
-          if (j >= vectors) continue;
-          const V16 v = xv[j];
-#pragma unroll
-          for (int e = VEC - 1; e >= 0; --e) {
-            const float f = to_f<T>(v.v[e]);
-            if (order_of(f) == floor) k[i] = key_of(f, parts.head + (int64_t)j * VEC + e);
-          }
-        }
-      }
-      ts.cand[column] = k[i];
-      const unsigned more = __ballot_sync(kAll, value[i] > floor);
-      if ((tid & 31) == 0) atomicAdd(&ts.larger, __popc(more));
-    }
-    __syncthreads();
-    if (tid == 0) ts.n_won = 0;
-    const int need = p.top - ts.larger;  // so many of the equal ones
-    int r[2] = {0, 0};
-    for (int i = 0; i < kColumns; ++i) {
-      r[0] += ts.cand[i] > k[0];
-      r[1] += ts.cand[i] > k[1];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      push_winner(ts, value[i] > floor || (k[i] != kNoKey && r[i] < need), tid + i * kSelThreads);
-      if (k[i] != kNoKey && r[i] == need - 1) ts.threshold = k[i];
-    }
-    __syncthreads();
-    won = ts.n_won;
-    threshold = need > 0 ? ts.threshold : (long long)(floor + 1) * 0x100000000ll;
-  }
-
-  const float floor_value = threshold == kNoKey ? -INFINITY : key_value(threshold);
-  auto offer = [&](float f, int64_t index) {
-    if (f < floor_value) return;
-    const long long k = key_of(f, index);
-    if (k < threshold) return;
-    const int at = atomicAdd(&ts.n_cand, 1);
-    if (at < kCandidates) ts.cand[at] = k;
-  };
-  const int64_t last_equal = key_index(threshold);  // values that equal the bound count up to here
-  const unsigned todo = (unsigned)won << column_log;
-  for (unsigned i = tid; i < todo; i += kUnroll * kSelThreads) {
-    V16 v[kUnroll];
-    unsigned at[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const unsigned q = i + u * kSelThreads;
-      at[u] = q < todo ? vector_of(ts.winners[q >> column_log], q & ((1u << column_log) - 1)) : vectors;
-      if (at[u] < vectors) v[u] = xv[at[u]];
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (at[u] >= vectors) continue;
-      const V16 one[1] = {v[u]};
-      const float vm = largest<T>(one);
-      if (vm < floor_value || (vm == floor_value && parts.head + (int64_t)at[u] * VEC > last_equal)) continue;
-      const int h = atomicAdd(&ts.n_hit, 1);
-      if (h >= kHits) continue;
-      ts.hit[h] = *reinterpret_cast<const uint4*>(&v[u]);
-      ts.hit_at[h] = (int)at[u];
-    }
-  }
-  __syncthreads();
-  const int hits = ts.n_hit;
-  for (int i = tid; i < min(hits, kHits) * VEC; i += kSelThreads)
-    offer(to_f<T>(reinterpret_cast<const T*>(ts.hit)[i]), parts.head + (int64_t)ts.hit_at[i / VEC] * VEC + i % VEC);
-  // the row's ends, at most 2 (VEC - 1) values
-  const int64_t end_at = tid < parts.head ? tid : parts.tail0 + (tid - parts.head);
-  const bool end = end_at < p.V && tid < parts.head + (p.V - parts.tail0);
-  if (end) offer(to_f<T>(x[end_at]), end_at);
-  __syncthreads();
-
-  auto put = [&](int i, long long k) {
-    p.top_ids[row * p.top + i] = key_index(k);
-    p.top_lp[row * p.top + i] = l2s == -INFINITY ? -INFINITY : (key_value(k) - m) * p.inv_tau - l2s * kLn2;
-  };
-  const int n = ts.n_cand;
-  if (hits <= kHits && n <= kCandidates) {
-    // each candidate's place is the number of larger ones, which 4 threads count
-    const int part = tid & 3;
-    for (int i0 = 0; i0 < n; i0 += kSelThreads / 4) {
-      const int i = i0 + (tid >> 2);
-      const long long k = i < n ? ts.cand[i] : kNoKey;
-      int r = 0;
-#pragma unroll 4
-      for (int j = part; j < n; j += 4) r += ts.cand[j] > k;
-      r += __shfl_xor_sync(kAll, r, 1);
-      r += __shfl_xor_sync(kAll, r, 2);
-      if (part == 0 && i < n && r < p.top) put(r, k);
-    }
-    return;
-  }
-  // More values above the bound than there is room for: rows whose largest values all lie in a few columns. Takes the
-  // largest key below the last one, k times over.
-  long long last = LLONG_MAX;
-  for (int i = 0; i < p.top; ++i) {
-    long long k = kNoKey;
-    for (int64_t j = tid; j < parts.vectors; j += kSelThreads) {
-      const V16 v = xv[j];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const long long q = key_of(to_f<T>(v.v[e]), parts.head + j * VEC + e);
-        if (q < last) k = max(k, q);
-      }
-    }
-    if (end) {
-      const long long q = key_of(to_f<T>(x[end_at]), end_at);
-      if (q < last) k = max(k, q);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) k = max(k, __shfl_xor_sync(kAll, k, o));
-    __syncthreads();
-    if ((tid & 31) == 0) ts.red[tid >> 5] = k;
-    __syncthreads();
-    for (int w = 0; w < kSelThreads / 32; ++w) k = max(k, ts.red[w]);
-    if (tid == 0) put(i, k);
-    last = k;
+    pick_top<T, NT>(top, x, parts, row, all.m, all.s, ts);
   }
 }
 
@@ -758,6 +780,14 @@ void token_logprobs_fwd_launch(const at::Tensor& logits, const at::Tensor& token
     maxima = at::Tensor(at::detail::empty_cuda({rows, (int64_t)g.stride}, at::kFloat, logits.device(), c10::nullopt));
     p.maxima = maxima.data_ptr<float>();
   }
+  // With a CTA or less on each SM the alternatives are picked where the row was read: a launch less (4 x 50304 bf16,
+  // k = 8: 6.6 us on the device, as two kernels 7.8 us, and 3.5 us less on the host). With more, they would wait behind the other rows' loads.
+  const bool here = top > 0 && !warp && rows * C <= num_sms();
+  TopParams q{p.maxima, nullptr, nullptr, p.inv_tau, (int)top, p.groups};
+  if (top > 0) {
+    q.top_lp = top_lp.data_ptr<float>();
+    q.top_ids = top_ids.data_ptr<int64_t>();
+  }
   auto launch = [&](auto kernel) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(warp ? ceil_div(rows, kThreads / 32) : rows * C));
@@ -769,31 +799,33 @@ void token_logprobs_fwd_launch(const at::Tensor& logits, const at::Tensor& token
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = C > 1 ? 1 : 0;
-    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p, q));
     MT_LAUNCH_CHECK();
   };
   dispatch_act(logits.scalar_type(), [&](auto t) {
     using T = decltype(t);
-    auto with = [&](auto nt) {
-      constexpr int NT = decltype(nt)::value;
-      const bool ent = entropy.defined();
-      if (ent && top > 0)
-        launch(token_logprobs_fwd<T, true, true, NT>);
-      else if (ent)
-        launch(token_logprobs_fwd<T, true, false, NT>);
-      else if (top > 0)
-        launch(token_logprobs_fwd<T, false, true, NT>);
+    const bool ent = entropy.defined();
+    auto with = [&](auto nt, auto what) {
+      constexpr int NT = decltype(nt)::value, TOP = decltype(what)::value;
+      if (ent)
+        launch(token_logprobs_fwd<T, true, TOP, NT>);
       else
-        launch(token_logprobs_fwd<T, false, false, NT>);
+        launch(token_logprobs_fwd<T, false, TOP, NT>);
     };
-    if (warp)
-      with(std::integral_constant<int, 32>{});
+    using std::integral_constant;
+    if (warp && top > 0)
+      with(integral_constant<int, 32>{}, integral_constant<int, kTopMaxima>{});
+    else if (warp)
+      with(integral_constant<int, 32>{}, integral_constant<int, kNoTop>{});
+    else if (here)
+      with(integral_constant<int, kThreads>{}, integral_constant<int, kTopHere>{});
+    else if (top > 0)
+      with(integral_constant<int, kThreads>{}, integral_constant<int, kTopMaxima>{});
     else
-      with(std::integral_constant<int, kThreads>{});
-    if (top == 0) return;
-    TopParams q{p.logits, p.maxima, p.stats, top_lp.data_ptr<float>(), top_ids.data_ptr<int64_t>(), p.ld, V,
-                p.inv_tau, (int)top, p.groups};
-    token_logprobs_top<T><<<(unsigned)rows, kSelThreads, 0, cur_stream()>>>(q);
+      with(integral_constant<int, kThreads>{}, integral_constant<int, kNoTop>{});
+    if (top == 0 || here) return;
+    token_logprobs_top<T><<<(unsigned)rows, kTopThreads, 0, cur_stream()>>>(q, static_cast<const T*>(p.logits), p.ld, V,
+                                                                          p.stats);
     MT_LAUNCH_CHECK();
   });
 }
