@@ -135,7 +135,7 @@ std::vector<at::Tensor> rotary_raw(const std::vector<at::Tensor>& xs, const Rota
     outs.push_back(fresh_like(xs[i]));
     segs.push_back({tokens_of(in), tokens_of(outs[i]), heads_rot[i]});
   }
-  rotary_launch(segs, RotaryArgs{r.turns, r.rot_dim, r.interleaved, r.scale, positions, offset, inverse});
+  rotary_launch(segs, RotaryArgs{r.turns, r.rot_dim, r.interleaved, r.scale, positions, offset, inverse, false});
   return outs;
 }
 
@@ -245,9 +245,9 @@ void rotary_inplace(at::Tensor q, const OptTensor& k, const at::Tensor& turns, i
   c10::cuda::CUDAGuard guard(q.device());
   std::vector<RotarySegment> segs{{qt, qt, qt.size(2)}};
   if (kt.defined()) segs.push_back({tokens_of(kt), tokens_of(kt), kt.size(-2)});
-  rotary_launch(segs, RotaryArgs{turns, rot_dim, interleaved, scale, pos, offset, inverse});
-  q.unsafeGetTensorImpl()->bump_version();
+  q.unsafeGetTensorImpl()->bump_version();  // refuses inference tensors outside inference mode
   if (kt.defined()) kt.unsafeGetTensorImpl()->bump_version();
+  rotary_launch(segs, RotaryArgs{turns, rot_dim, interleaved, scale, pos, offset, inverse, true});
 }
 
 // ------------------------------------------------------------------------------------------ residual norm

@@ -25,6 +25,7 @@ struct RotaryArgs {
   OptTensor positions;  // int32 / int64 [B, S], any strides; none: offset + index in the sequence
   int64_t offset;
   bool inverse;
+  bool in_place;  // every segment's out is its in
 };
 void rotary_launch(const std::vector<RotarySegment>& segs, const RotaryArgs& a);
 

@@ -207,7 +207,7 @@ void rotary_launch(const std::vector<RotarySegment>& segs, const RotaryArgs& a) 
   }
   p.scale = (float)a.scale;
   p.sign = a.inverse ? -1.f : 1.f;
-  p.copy = segs[0].in.data_ptr() != segs[0].out.data_ptr();
+  p.copy = !a.in_place;
   if (p.tokens == 0 || p.heads == 0) return;
   dispatch_act(segs[0].in.scalar_type(), [&](auto t) {
     using T = decltype(t);

@@ -189,18 +189,19 @@ __device__ __forceinline__ void fast_add(Fast& a, const Vec<T, 16 / sizeof(T)>& 
   }
 }
 
-// The sums relative to the maximum itself; false where the values were out of range (a NaN or +inf among them shows
-// in the sums and needs no second look).
+// The sums relative to the maximum itself; false where the values were out of range, on the way to which the sums may
+// have overflowed. The reference only rises, so where it ended in range a NaN in the sums is one among the values.
 template <typename T, bool ENT>
 __device__ __forceinline__ bool fast_done(const Fast& a, float c, Running& out) {
   const float s = a.s.x + a.s.y, w = a.w.x + a.w.y;
   out = Running{kLowest, 0.f, 0.f};
+  if (fabsf(a.minus_r) > kFastLimit) return false;  // above the upper limit
   if (isnan(s)) {
     out.s = s;
     return true;
   }
   if (a.best == -INFINITY) return true;  // nothing, or masked values only
-  if (a.best < a.m || fabsf(a.minus_r) > kFastLimit) return false;  // below the lower limit, or above the upper
+  if (a.best < a.m) return false;        // below the lower limit
   if (ENT && (kept_above<T>() - a.m) * c > -200.f) return false;
   const float d = fmaf(a.m, c, a.minus_r), f = ex2(-d);
   out = Running{a.m, s * f, f * fmaf(-d, s, w)};

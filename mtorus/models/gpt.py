@@ -453,11 +453,17 @@ class GptModel(nn.Module):
         """Scores given continuations through the fused kernels: for each position the log
         probability of its target (a target outside the vocabulary is ignored), and on request
         the entropy and the ``top`` likeliest tokens (``mtorus.ops.logprobs.TokenLogprobs``,
-        [B, S] each).  bf16 LM head; records no gradient."""
+        [B, S] each).  Runs in bf16, without dropout, and records no gradient; FP8 scaling
+        histories and dropout keys of a training in progress stay as they are."""
         from ..ops import kernels as K
         from ..ops.logprobs import token_logprobs
 
-        h = self.fused_hidden(input_ids)
+        drop, fp8 = self.dropout_state, getattr(self, "fp8_state", None)
+        self.dropout_state = self.fp8_state = None
+        try:
+            h = self.fused_hidden(input_ids)
+        finally:
+            self.dropout_state, self.fp8_state = drop, fp8
         logits = K.gemm(h, self.lm_head.weight.w16, bias=self.lm_head.bias.data)
         return token_logprobs(logits.view(*targets.shape, self.vocab_size), targets, temperature=temperature, top=top,
                               entropy=entropy)

@@ -242,6 +242,31 @@ def test_rotary_empty():
     assert rotary_qkv(torch.empty(0, 12 * 64, device=DEV, dtype=BF), 0, 5, 4, rope).shape == (0, 12 * 64)
 
 
+def test_rotary_without_query_heads():
+    from mtorus.ops.rotary import rotary
+
+    rope = _rope(64, rot_dim=32)
+    k = torch.randn(3, 2, 64, generator=_gen(10), device=DEV)
+    q, got = rotary(torch.empty(3, 0, 64, device=DEV), k, rope)
+    assert q.shape == (3, 0, 64)
+    assert torch.equal(got, rotary(k, None, rope)[0]) and torch.equal(got[..., 32:], k[..., 32:])
+
+
+def test_rotary_inplace_and_inference_mode():
+    from mtorus.ops.rotary import rotary, rotary_
+
+    rope = _rope(64)
+    with torch.inference_mode():
+        q = torch.randn(3, 2, 64, device=DEV)
+        want, _ = rotary(q, None, rope)
+        rotary_(q, None, rope)
+        assert torch.equal(q, want)
+    before = q.clone()
+    with pytest.raises(RuntimeError, match="inference"):
+        rotary_(q, None, rope)
+    assert torch.equal(q, before)
+
+
 def test_rotary_gradient_of_one_side_only():
     from mtorus.ops.rotary import rotary
 
@@ -379,6 +404,19 @@ def test_residual_norm_gates(gate, dtype, d):
 def test_residual_norm_one_gradient_only(which):
     t, dy, dn = _norm_case(19, 512, BF, True, True, "channel", 3)
     _check_norm(t, dy if which == "y" else None, dn if which == "n" else None)
+
+
+@pytest.mark.parametrize("wanted", [("pre",), ("x",), ("h", "gate"), ("post", "gate"), ("x", "pre")])
+def test_residual_norm_some_gradients(wanted):
+    from mtorus.ops.residual_norm import residual_norm
+
+    t, dy, dn = _norm_case(50, 256, BF, True, True, "channel", 16)
+    ref = _ref_norm(t["x"], t["h"], t["pre"], t["post"], t["gate"], 1.0, 1.0, 1e-6, dy, dn)
+    leaf = {k: v.detach().requires_grad_(k in wanted) for k, v in t.items()}
+    y, n = residual_norm(leaf["x"], leaf["h"], pre_weight=leaf["pre"], post_weight=leaf["post"], gate=leaf["gate"])
+    got = torch.autograd.grad([y, n], [leaf[k] for k in wanted], [dy, dn], allow_unused=True)
+    for k, v in zip(wanted, got):
+        _close(v, *ref["d" + k], BWD_ROUNDINGS if k in "xh" else COL_ROUNDINGS, k)
 
 
 def test_residual_norm_many_rows():
@@ -730,6 +768,21 @@ def test_logprobs_peaked_and_extreme():
         _check_logprobs(x[keep], t[keep], tau=tau, top=3)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [3000, 70000])
+def test_logprobs_large_values_that_keep_rising(dtype, V):
+    """Each thread's maximum rises again and again far beyond where exponents are exact: still finite results."""
+    i = torch.arange(V, device=DEV).double()
+    x = torch.stack([1e30 * (1 + i), 1e32 * (1 + i / V), -1e30 * (V - i), 1e9 + 1e7 * i, i * 0 + 3e38]).to(dtype)
+    for rows in (slice(0, 5), slice(0, 1)):
+        xr = x[rows]
+        t = torch.randint(0, V, (xr.shape[0],), generator=_gen(13), device=DEV)
+        t[0] = V - 1
+        for ent in (True, False):
+            r = _check_logprobs(xr, t, top=4, entropy=ent)
+            assert torch.isfinite(r.logprob).all()
+
+
 @pytest.mark.parametrize("grads", ["l", "h", "k", "lk", "hk"])
 def test_logprobs_parts_of_the_gradient(grads):
     x, t = _logits(9, 2051, BF, 5)
@@ -1031,3 +1084,13 @@ def test_model_scores_tokens():
     assert (r.logprob - want).abs().max() <= 16 * 2.0 ** -9 * 4
     assert (r.top_logprobs[..., 0] - lp.amax(-1)).abs().max() <= 16 * 2.0 ** -9 * 4
     assert not r.logprob.requires_grad
+    # in the middle of a training with dropout and FP8: the same scores, and the training's state untouched
+    model.config.dropout = 0.5
+    model.enable_dropout(3)
+    model.enable_fp8(recipe="tensor")
+    key, cursor = model.dropout_state.rng.clone(), model.fp8_state.state_dict()
+    again = model.fused_token_logprobs(ids[:, :-1], tgt, top=5, entropy=True)
+    assert all(torch.equal(a, b) for a, b in zip(r, again))
+    assert torch.equal(key, model.dropout_state.rng)
+    after = model.fp8_state.state_dict()
+    assert str(after) == str(cursor)
