@@ -9,12 +9,15 @@
 //
 // Bound by memory: forward 2 reads and 2 writes of [T, d], backward 4 and 2.  One CTA of d / 8 threads walks a
 // strided set of rows; a thread owns the same 8 columns of every row, so the weights and the sums of weight
-// gradients stay in its registers.  Its vectors of the next rows are on their way through a ring in shared memory;
+// gradients stay in its registers (16 columns, half the threads, above d = 4096).  Its vectors of the next rows are on their way through a ring in shared memory;
 // each thread reads back only what it copied itself, so the ring needs no barrier.
 //
 // The backward needs little more than the memory's time in instructions, so it is written to need few: one row
 // reduction, not two (mean(e hh Y) follows from sums of e hh with dy + ry u and with yh), one column sum q = sum r Y hh for
 // both dpost = alpha g q and dgate = alpha post q, pairs of values per instruction, and 6 shuffles for 3 row sums.
+//
+// 16384 x 2048 bf16, both norms and a gate per channel: forward 45 us (a bare stream of its reads and writes takes as
+// long), backward 73 us (63 us) and 4.5 us for the weights' sums; the copy's rate allows 41 us and 62 us.
 #include <ATen/cuda/EmptyTensor.h>
 
 #include "decoder_ops.h"
