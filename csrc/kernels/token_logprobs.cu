@@ -548,11 +548,7 @@ __global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : TOP == kTopHere ? 2 :
   const RowParts<T> parts(x, p.V);
   const V16* xv = reinterpret_cast<const V16*>(x + parts.head);
   int64_t token = -1;
-  float token_value = 0.f;
-  if (rank == 0 && tid == 0) {
-    token = p.tokens[row];
-    if (token >= 0 && token < p.V) token_value = to_f<T>(x[token]);
-  }
+  if (rank == 0 && tid == 0) token = p.tokens[row];  // looked at after the loop: nothing may wait before its loads
 
   // one pass, a tile after the other
   const int64_t tiles = (parts.vectors + TILE - 1) / TILE;
@@ -590,6 +586,8 @@ __global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : TOP == kTopHere ? 2 :
     const float vm = take(v);
     if constexpr (TOP != kNoTop) keep(v, tile, vm);
   }
+  T token_value = from_f<T>(0.f);
+  if (token >= 0 && token < p.V) token_value = x[token];
   if (tile < tiles) {  // the last one, where it is not full
     const int64_t j = tile * TILE + tid;
     V16 v[kUnroll];
@@ -644,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : TOP == kTopHere ? 2 :
     const bool none = a.s == 0.f;
     const float l2s = none ? -INFINITY : log2f(a.s);
     float lp = 0.f;
-    if (token >= 0 && token < p.V) lp = none ? -INFINITY : (token_value - a.m) * p.inv_tau - l2s * kLn2;
+    if (token >= 0 && token < p.V) lp = none ? -INFINITY : (to_f<T>(token_value) - a.m) * p.inv_tau - l2s * kLn2;
     p.logprob[row] = lp;
     p.stats[2 * row] = a.m;
     p.stats[2 * row + 1] = l2s;
