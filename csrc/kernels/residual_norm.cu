@@ -7,9 +7,9 @@
 // y is computed again from x and h in 32 bits (reading x instead of y costs the same bytes), so the statistics
 // and the weight gradients see the value before its rounding.
 //
-// Bound by memory: forward 2 reads and 2 writes of [T, d], backward 4 and 2.  One CTA of d / 8 threads walks a
-// strided set of rows; a thread owns the same 8 columns of every row, so the weights and the sums of weight
-// gradients stay in its registers (16 columns, half the threads, above d = 4096).  Its vectors of the next rows are on their way through a ring in shared memory;
+// Bound by memory: forward 2 reads and 2 writes of [T, d], backward 4 and 2.  One CTA of d / 8 threads (or
+// d / 16) walks a strided set of rows; a thread owns the same 8 (16) columns of every row, so the weights and the sums of weight
+// gradients stay in its registers.  Its vectors of the next rows are on their way through a ring in shared memory;
 // each thread reads back only what it copied itself, so the ring needs no barrier.
 //
 // The backward needs little more than the memory's time in instructions, so it is written to need few: one row
@@ -17,7 +17,7 @@
 // both dpost = alpha g q and dgate = alpha post q, pairs of values per instruction, and 6 shuffles for 3 row sums.
 //
 // 16384 x 2048 bf16, both norms and a gate per channel: forward 45 us (a bare stream of its reads and writes takes as
-// long), backward 73 us (63 us) and 4.5 us for the weights' sums; the copy's rate allows 41 us and 62 us.
+// long), backward 71 us (63 us) and 4.5 us for the weights' sums; the copy's rate allows 41 us and 62 us.
 #include <ATen/cuda/EmptyTensor.h>
 
 #include "decoder_ops.h"
@@ -482,7 +482,9 @@ struct Shape {
   int threads, groups, ins;
 };
 
-Shape shape_of(const NormParams& p, int esize) {
+// wide_from: 256-column groups in an aligned row from which a thread takes two of them.
+constexpr int kWide = 17;  // more do not fit the registers of a CTA's threads otherwise
+Shape shape_of(const NormParams& p, int esize, int wide_from) {
   const int v = 16 / esize;
   bool ok = true;
   int ins = 0;
@@ -495,7 +497,7 @@ Shape shape_of(const NormParams& p, int esize) {
   if (p.gate_kind == kGateFull) ok = ok && reinterpret_cast<uintptr_t>(p.dgate) % 16 == 0;
   Shape s{!ok ? kSingle : p.d % v == 0 ? kAligned : kShifted, 0, 0, ins};
   const int per = (p.d + (s.mode == kShifted ? v - 1 : 0) + 255) / 256;
-  s.groups = per > kMaxWarps / 2 ? 2 : 1;
+  s.groups = per >= (s.mode == kAligned ? wide_from : kWide) ? 2 : 1;
   s.threads = (per + s.groups - 1) / s.groups * 32;
   // a row has to fit into the ring, and into a CTA
   if (s.mode != kSingle && (ins * s.groups * s.threads * 8 * esize > kSmemBudget || s.threads > 1024)) {
@@ -512,8 +514,10 @@ void with_shape(const Shape& s, bool all, F&& f) {
   auto go = [&](auto mode, auto every) {
     if (s.groups == 2 && s.threads > 512)
       f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 1024>{});
-    else if (s.groups == 2)
+    else if (s.groups == 2 && s.threads > 256)
       f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 512>{});
+    else if (s.groups == 2)
+      f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 256>{});
     else if (s.threads > 256)
       f(mode, integral_constant<int, 1>{}, every, integral_constant<int, 512>{});
     else
@@ -549,6 +553,17 @@ int64_t plan_ring(NormParams& p, const Shape& s, int esize, int fit, int deepest
     fit = std::max(1, std::min(fit, kSmemBudget / (p.stage * p.depth)));
   }
   return (int64_t)num_sms() * fit;
+}
+
+// CTAs of this size that an SM's registers (four files of 16384, a warp in one of them) hold, at most 16.
+template <auto KERNEL>
+int fit_of(int threads) {
+  static const int warps = [] {
+    cudaFuncAttributes a{};
+    C10_CUDA_CHECK(cudaFuncGetAttributes(&a, KERNEL));
+    return 4 * (16384 / ((a.numRegs + 7) / 8 * 8 * 32));
+  }();
+  return std::max(1, std::min(16, warps * 32 / threads));
 }
 
 template <typename K>
@@ -602,13 +617,14 @@ void residual_norm_fwd_launch(const ResidualNormArgs& a, const at::Tensor& y, co
   if (p.rows == 0) return;
   dispatch_act(a.x.scalar_type(), [&](auto t) {
     using T = decltype(t);
-    const Shape s = shape_of(p, sizeof(T));
+    const Shape s = shape_of(p, sizeof(T), kWide);
     const bool all = p.in[kH] != nullptr && p.n != nullptr && a.gate_kind != kGateFull;
     with_shape(s, all, [&](auto mode, auto ng, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 1024 ? 1 : 1024 / kMaxT;
-      const int fit = std::min(16, kMinB * kMaxT / s.threads);
-      const unsigned grid = grid_of(plan_ring(p, s, sizeof(T), fit, 4), p, s, sizeof(T));
-      launch_norm(residual_norm_fwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, grid);
+      constexpr auto kernel =
+          residual_norm_fwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>;
+      const int64_t resident = plan_ring(p, s, sizeof(T), fit_of<kernel>(s.threads), 4);
+      launch_norm(kernel, p, s, grid_of(resident, p, s, sizeof(T)));
     });
   });
 }
@@ -638,13 +654,17 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
   }
   dispatch_act(a.x.scalar_type(), [&](auto t) {
     using T = decltype(t);
-    const Shape s = shape_of(p, sizeof(T));
     bool all = a.gate_kind != kGateFull;
     for (const void* q : {p.in[kH], p.in[kDy], p.in[kDn], (const void*)p.dx, (const void*)p.dh}) all = all && q != nullptr;
+    // Two groups for a thread from d = 1025 on: with a barrier for every row, 4 warps that do more each and 8 of them on
+    // an SM do better than 16 (16384 x 2048 bf16 71.4 us against 73.5 us, 4096 x 4096 40.3 us against 42 us). The kernel
+    // for any set of inputs needs too many registers for that (8192 x 2048 with a gate per element 64 us against 57 us).
+    const Shape s = shape_of(p, sizeof(T), all ? 5 : kWide);
     with_shape(s, all, [&](auto mode, auto ng, auto every, auto maxt) {
-      constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 256 ? 2 : 1;
-      const int fit = std::min(16, kMinB * kMaxT / s.threads);
-      int64_t grid = plan_ring(p, s, sizeof(T), fit, 4);
+      constexpr int kMaxT = decltype(maxt)::value, kMinB = decltype(ng)::value == 1 && kMaxT == 256 ? 2 : 1;
+      constexpr auto kernel =
+          residual_norm_bwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>;
+      int64_t grid = plan_ring(p, s, sizeof(T), fit_of<kernel>(s.threads), 4);
       // a few rows for each CTA at least: its partial sums cost as much as two rows
       if (p.want_dpre || p.want_q) grid = std::min<int64_t>(grid, (p.rows + 3) / 4);
       grid = grid_of(grid, p, s, sizeof(T));
@@ -653,7 +673,7 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
         part = at::Tensor(at::detail::empty_cuda({grid, 2, (int64_t)p.d}, at::kFloat, a.x.device(), c10::nullopt));
         p.part = part.data_ptr<float>();
       }
-      launch_norm(residual_norm_bwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>, p, s, (unsigned)grid);
+      launch_norm(kernel, p, s, (unsigned)grid);
       if (p.part != nullptr) {
         residual_norm_finish<<<dim3((p.d + 31) / 32, p.want_dpre + p.want_q), kFinishWarps * 32, 0, cur_stream()>>>(
             p.part, (int)grid, p.d, p.want_dpre, p.alpha, a.gate_kind == kGateChannel ? p.gate : nullptr, p.post,
