@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <cstdlib>
 #include <tuple>
 
 #include "kernels/decoder_ops.h"
@@ -29,6 +30,10 @@ void check_act(const at::Tensor& t, const char* op, const char* name) {
 // Last of the checks, so that every other refusal can be had without a GPU.
 void check_cuda(std::initializer_list<const at::Tensor*> ts, const char* op) {
   const at::Tensor* first = nullptr;
+  for (const at::Tensor* t : ts) {
+    if (t->defined())
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), op, ": no forward-mode gradient");
+  }
   for (const at::Tensor* t : ts) {
     if (!t->defined()) continue;
     TORCH_CHECK(t->is_cuda(), op, ": the tensors must be on a CUDA device (one is on ", t->device(), ")");
@@ -179,6 +184,24 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
   }
 };
 
+// Whether a token's heads of q and of k lie over one another, as two views of a packed matrix may. (Views that are not
+// dense as a whole are beyond at::assert_no_overlap.)
+bool share_heads(const at::Tensor& q, const at::Tensor& k) {
+  const int64_t n = q.dim(), D = q.size(-1), step = q.stride(-2);
+  if (q.numel() == 0 || k.numel() == 0 || !q.is_alias_of(k) || (k.size(-2) > 1 && q.size(-2) > 1 && k.stride(-2) != step))
+    return false;
+  for (int64_t i = 0; i < n - 2; ++i) {
+    if (q.size(i) > 1 && q.stride(i) != k.stride(i)) return false;
+  }
+  const int64_t between = k.storage_offset() - q.storage_offset();
+  const int64_t stride = q.size(-2) > 1 ? step : k.size(-2) > 1 ? k.stride(-2) : D;
+  // head j of k starts (between + (j - i) stride) values after head i of q
+  for (int64_t m = 1 - q.size(-2); m < k.size(-2); ++m) {
+    if (std::abs(between + m * stride) < D) return true;
+  }
+  return false;
+}
+
 }  // namespace
 
 std::tuple<at::Tensor, OptTensor> rotary(const at::Tensor& q, const OptTensor& k, const at::Tensor& turns,
@@ -229,7 +252,7 @@ void rotary_inplace(at::Tensor q, const OptTensor& k, const at::Tensor& turns, i
   for (const at::Tensor* t : {&q, &kt}) {
     if (!t->defined()) continue;
     check_rotary(*t, t == &q ? "q" : "k", r);
-    TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()),
+    TORCH_CHECK(!needs_grad({t}),
                 "rotary_: works in place and records no gradient; use rotary() on tensors that require one");
     TORCH_CHECK_VALUE(t->size(-1) <= 1 || t->stride(-1) == 1, "rotary_: the head dim must have stride 1");
     at::assert_no_internal_overlap(*t);
@@ -238,6 +261,7 @@ void rotary_inplace(at::Tensor q, const OptTensor& k, const at::Tensor& turns, i
     check_pair(q, kt);
     TORCH_CHECK_VALUE(q.data_ptr() != kt.data_ptr() || q.numel() == 0, "rotary_: q and k are the same memory");
     at::assert_no_overlap(q, kt);
+    TORCH_CHECK_VALUE(!share_heads(q, kt), "rotary_: q and k are the same memory in some of their heads");
   }
   const at::Tensor qt = tokens_of(q);
   const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1));

@@ -97,6 +97,26 @@ def test_rotary_inplace_refuses():
         rotary_(q, None, rope)
 
 
+def _packed_heads(q_from, q_to, k_from, k_to, heads_first=False):
+    rope = _rope()
+    packed = torch.zeros(2, 8, 5, 64, dtype=BF).transpose(1, 2) if heads_first else torch.zeros(2, 5, 8, 64, dtype=BF)
+    rotary_(packed[:, :, q_from:q_to], packed[:, :, k_from:k_to], rope)
+
+
+@pytest.mark.parametrize("heads_first", [False, True])
+@pytest.mark.parametrize("heads", [(0, 4, 3, 5), (0, 4, 0, 2), (2, 4, 0, 3), (3, 4, 0, 8), (0, 8, 7, 8)])
+def test_rotary_inplace_refuses_heads_in_common(heads, heads_first):
+    with pytest.raises(ValueError, match="same memory"):
+        _packed_heads(*heads, heads_first)
+
+
+@pytest.mark.parametrize("heads_first", [False, True])
+@pytest.mark.parametrize("heads", [(0, 4, 4, 6), (4, 8, 0, 4), (0, 1, 1, 8), (7, 8, 6, 7)])
+def test_rotary_inplace_takes_heads_side_by_side(heads, heads_first):
+    with pytest.raises(RuntimeError, match="CUDA"):  # the last check: without a GPU nothing runs
+        _packed_heads(*heads, heads_first)
+
+
 def test_causal_attention_rotary_refuses():
     qkv = torch.zeros(128, 3 * 128, dtype=BF)
     with pytest.raises(ValueError, match="head dim 64"):
@@ -158,3 +178,21 @@ def test_token_logprobs_refuses():
             token_logprobs(x, t, temperature=tau)
     with pytest.raises(RuntimeError, match="CUDA"):
         token_logprobs(x, t, top=4, entropy=True)
+
+
+def test_forward_mode_gradients_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    rope, w = _rope(), torch.ones(64)
+    x = torch.zeros(5, 4, 64)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        calls = [lambda: rotary(dual, None, rope), lambda: rotary(x, dual, rope), lambda: rotary_(dual, None, rope),
+                 lambda: rotary_qkv(dual.reshape(5, 256), 1, 5, 2, rope, kv_heads=1),
+                 lambda: residual_norm(x, dual, pre_weight=w),
+                 lambda: residual_norm(x, x, pre_weight=fwd.make_dual(w, w)),
+                 lambda: rms_norm(dual, w),
+                 lambda: token_logprobs(dual, torch.zeros(5, 4, dtype=torch.int64))]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
