@@ -10,7 +10,8 @@
 // Bound by memory: forward 2 reads and 2 writes of [T, d], backward 4 and 2.  One CTA of d / 8 threads (or
 // d / 16) walks a strided set of rows; a thread owns the same 8 (16) columns of every row, so the weights and the sums of weight
 // gradients stay in its registers.  Its vectors of the next rows are on their way through a ring in shared memory;
-// each thread reads back only what it copied itself, so the ring needs no barrier.
+// each thread reads back only what it copied itself, so the ring needs no barrier. Rows of up to 128 columns (the norm
+// of a head) share a warp.
 //
 // The backward needs little more than the memory's time in instructions, so it is written to need few: one row
 // reduction, not two (mean(e hh Y) follows from sums of e hh with dy + ry u and with yh), one column sum q = sum r Y hh for
@@ -53,20 +54,22 @@ struct NormParams {
 enum Mode : int { kSingle, kAligned, kShifted };
 
 // Place in its row, counted from the first vector's start, of a thread's i-th value in a group of 256: vectors, or single
-// values 32 apart, so that each load of the warp is contiguous.
-template <typename T, int MODE>
+// values 32 apart, so that each load of the warp is contiguous. LANES < 32: lanes of a warp that share a row of at most
+// 8 LANES columns, in one group.
+template <typename T, int MODE, int LANES>
 __device__ __forceinline__ int place_of(int group, int lane, int i) {
   constexpr int VEC = 16 / sizeof(T);
   if constexpr (MODE == kSingle) return group * 256 + i * 32 + lane;
-  return group * 256 + (i / VEC) * (32 * VEC) + lane * VEC + i % VEC;
+  return group * 256 + (i / VEC) * (LANES * VEC) + lane * VEC + i % VEC;
 }
 
 // The rows that a thread has asked for, and their values. The slots of one row lie one input after another, each
 // with one 16-byte vector of every thread after the other. INPUTS: a bit for each input, or 0 where the kernel looks
 // at its parameters for which ones there are.
-template <typename T, int MODE, int NG, unsigned INPUTS>
+template <typename T, int MODE, int NG, int LANES, unsigned INPUTS>
 struct Rows {
-  static constexpr int VEC = 16 / sizeof(T), NV = 8 / VEC;
+  static_assert(LANES == 32 || (MODE == kAligned && NG == 1), "several rows to a warp");
+  static constexpr int VEC = 16 / sizeof(T), NV = 8 / VEC, PER = 32 / LANES;  // PER: rows at a time
   const NormParams& p;
   const unsigned char* mine;  // this thread's first vector in the ring
   uint32_t address;           // the same as a shared-memory address
@@ -77,13 +80,25 @@ struct Rows {
       : p(p),
         mine(ring + threadIdx.x * 16),
         address(static_cast<uint32_t>(__cvta_generic_to_shared(mine))),
-        lane(threadIdx.x & 31),
+        lane(threadIdx.x & (LANES - 1)),
         g0((threadIdx.x >> 5) * NG),
         pitch(blockDim.x * 16),
         shift(MODE == kShifted ? (int)((uint64_t)blockIdx.x * p.d % VEC) : 0) {}
 
   // column of a thread's i-th value; below 0 or from d on: none
-  __device__ __forceinline__ int column(int g, int i) const { return place_of<T, MODE>(g0 + g, lane, i) - shift; }
+  __device__ __forceinline__ int column(int g, int i) const { return place_of<T, MODE, LANES>(g0 + g, lane, i) - shift; }
+
+  // the CTA's first rows, and from one set of rows to the next; `mine`: the thread's row of a set, which may lie behind
+  // the last one where PER > 1
+  __device__ __forceinline__ uint32_t first() const { return blockIdx.x * PER; }
+  __device__ __forceinline__ uint32_t step() const { return gridDim.x * PER; }
+  __device__ __forceinline__ uint32_t mine_of(uint32_t set) const {
+    return LANES == 32 ? set : set + (threadIdx.x & 31) / LANES;
+  }
+  __device__ __forceinline__ bool there(uint32_t row) const { return LANES == 32 || row < p.rows; }
+  __device__ __forceinline__ bool leads(uint32_t row) const {  // the thread that writes the row's scalars
+    return LANES == 32 ? threadIdx.x == 0 : lane == 0 && row < p.rows;
+  }
 
   __device__ __forceinline__ bool has(int t) const { return INPUTS != 0 ? INPUTS >> t & 1 : p.in[t] != nullptr; }
 
@@ -93,17 +108,19 @@ struct Rows {
 
   __device__ __forceinline__ void ask(uint32_t row, int stage) const {
     if constexpr (MODE != kSingle) {
-      if (row < p.rows) {
+      if (LANES < 32 || row < p.rows) {
 #pragma unroll
         for (int t = 0; t < kIns; ++t) {
           if (!has(t)) continue;
-          const T* src = row_of(t, row) - shift;
+          // a row that is not there is zeros, so that the other rows' column sums stay clean
+          const T* src = row_of(t, there(row) ? row : 0) - shift;
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
               // what lies behind the row is not read: zeros take its place
-              const int at = place_of<T, MODE>(g0 + g, lane, k * VEC), left = p.d + shift - at;
+              const int at = place_of<T, MODE, LANES>(g0 + g, lane, k * VEC),
+                        left = there(row) ? p.d + shift - at : 0;
               const int bytes = MODE == kAligned ? (left > 0 ? 16 : 0) : max(0, min(16, left * (int)sizeof(T)));
               copy_async16(address + stage * p.stage + p.slot[t] + (g * NV + k) * pitch, src + (left > 0 ? at : 0),
                            bytes);
@@ -166,7 +183,7 @@ struct Rows {
           w = make_uint4(__float_as_uint(f[2 * k].x), __float_as_uint(f[2 * k].y), __float_as_uint(f[2 * k + 1].x),
                          __float_as_uint(f[2 * k + 1].y));
         }
-        if (MODE == kAligned ? c < p.d : c >= 0 && c + VEC <= p.d) {
+        if (MODE == kAligned ? c < p.d && there(row) : c >= 0 && c + VEC <= p.d) {
           __stcs(reinterpret_cast<uint4*>(dst + c), w);
         } else if (MODE == kShifted) {  // the row's ends
 #pragma unroll
@@ -204,9 +221,15 @@ struct Rows {
   }
 };
 
-// Sum of one value over the CTA for every thread. `red` holds [2][kMaxWarps] floats; `par` alternates between its
+// Sum of one value over the CTA (LANES < 32: over the lanes of a row) for every thread. `red` holds [2][kMaxWarps] floats; `par` alternates between its
 // halves, so that one barrier per call is enough.
+template <int LANES>
 __device__ __forceinline__ float cta_sum(float v, float* red, int& par) {
+  if constexpr (LANES < 32) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
   v = warp_sum(v);
   const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
   if (nw == 1) return v;
@@ -219,8 +242,18 @@ __device__ __forceinline__ float cta_sum(float v, float* red, int& par) {
 
 // The same for three values; `red` holds [2][kMaxWarps] float4. Halves and quarters of the warp first share the values
 // out among them, so that 6 shuffles do; then a lane adds one value of every 8th warp.
+template <int LANES>
 __device__ __forceinline__ float3 cta_sum3(float3 v, float4* red, int& par) {
   constexpr unsigned kAll = 0xffffffffu;
+  if constexpr (LANES < 32) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(kAll, v.x, o);
+      v.y += __shfl_xor_sync(kAll, v.y, o);
+      v.z += __shfl_xor_sync(kAll, v.z, o);
+    }
+    return v;
+  }
   const int lane = threadIdx.x & 31;
   const bool up = lane & 16, odd = lane & 8;
   const float a = (up ? v.z : v.x) + __shfl_xor_sync(kAll, up ? v.x : v.z, 16);
@@ -247,11 +280,11 @@ __device__ __forceinline__ float3 cta_sum3(float3 v, float4* red, int& par) {
 
 // ALL: there are a branch and a pre norm, and no gate per element -- what a training step calls; with this known, and
 // the rest done by arithmetic (no post norm is rh = 1), a row takes two thirds of the instructions.
-template <typename T, int MODE, int NG, bool ALL, int MAXT, int MINB>
+template <typename T, int MODE, int NG, int LANES, bool ALL, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[2 * kMaxWarps];
-  const Rows<T, MODE, NG, ALL ? 1u << kX | 1u << kH : 0u> in(p, ring);
+  const Rows<T, MODE, NG, LANES, ALL ? 1u << kX | 1u << kH : 0u> in(p, ring);
   const float inv_d = 1.f / p.d;
   const bool branch = in.has(kH);
   int par = 0, stage = 0;
@@ -263,15 +296,16 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
   }
   float gates = 1.f;  // of the CTA's next 32 rows, one row per lane
   int turn = 0;
-  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + k * gridDim.x, k);
-  for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    in.ask(row + (p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
+  for (int k = 0; k < p.depth - 1; ++k) in.ask(in.mine_of(in.first() + k * in.step()), k);
+  for (uint32_t set = in.first(); set < p.rows; set += in.step()) {
+    const uint32_t row = in.mine_of(set);
+    in.ask(row + (p.depth - 1) * in.step(), stage == 0 ? p.depth - 1 : stage - 1);
     float gate = 1.f;
     if (p.gate_kind == kGateRow) {
-      const uint64_t mine = row + (uint64_t)in.lane * gridDim.x;
+      const uint64_t mine = row + (uint64_t)in.lane * in.step();
       if (turn == 0 && mine < p.rows) gates = p.gate[mine];
-      gate = __shfl_sync(0xffffffffu, gates, turn);
-      turn = (turn + 1) & 31;
+      gate = __shfl_sync(0xffffffffu, gates, turn, LANES);
+      turn = (turn + 1) & (LANES - 1);
     }
     if constexpr (MODE != kSingle) copy_async_wait(p.depth - 1);
     float2 y[NG][4];
@@ -285,8 +319,8 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
         for (int g = 0; g < NG; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s = fma2(y[g][i], y[g][i], s);
-        rh = rsqrtf(cta_sum(s.x + s.y, red, par) * inv_d + p.eps);
-        if (threadIdx.x == 0 && p.rstd_h != nullptr) p.rstd_h[row] = rh;
+        rh = rsqrtf(cta_sum<LANES>(s.x + s.y, red, par) * inv_d + p.eps);
+        if (in.leads(row) && p.rstd_h != nullptr) p.rstd_h[row] = rh;
       }
       const float2 r = both(rh * gate), beta = both(p.beta);
 #pragma unroll
@@ -315,8 +349,8 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s = fma2(y[g][i], y[g][i], s);
-      const float ry = rsqrtf(cta_sum(s.x + s.y, red, par) * inv_d + p.eps);
-      if (threadIdx.x == 0 && p.rstd_y != nullptr) p.rstd_y[row] = ry;
+      const float ry = rsqrtf(cta_sum<LANES>(s.x + s.y, red, par) * inv_d + p.eps);
+      if (in.leads(row) && p.rstd_y != nullptr) p.rstd_y[row] = ry;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
 #pragma unroll
@@ -331,11 +365,11 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_fwd(const __grid_con
 
 // part: [gridDim.x][2][d], the CTA's sums of dn yh (dpre) and of r Y hh (q; with the gate of each element)
 // ALL: as in the forward, and both gradients come in and both are wanted.
-template <typename T, int MODE, int NG, bool ALL, int MAXT, int MINB>
+template <typename T, int MODE, int NG, int LANES, bool ALL, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float4 red[2 * kMaxWarps];
-  const Rows<T, MODE, NG, ALL ? 1u << kX | 1u << kH | 1u << kDy | 1u << kDn : 0u> in(p, ring);
+  const Rows<T, MODE, NG, LANES, ALL ? 1u << kX | 1u << kH | 1u << kDy | 1u << kDn : 0u> in(p, ring);
   const float inv_d = 1.f / p.d;
   const bool branch = in.has(kH), full = !ALL && p.gate_kind == kGateFull, post = p.post != nullptr;
   int par = 0, stage = 0;
@@ -351,11 +385,12 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
   // each row would be late each time: 81 us against 73 us at 16384 x 2048 bf16.
   float rhs = 1.f, rys = 0.f, gates = 1.f;
   int turn = 0;
-  for (int k = 0; k < p.depth - 1; ++k) in.ask(blockIdx.x + k * gridDim.x, k);
-  for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    in.ask(row + (p.depth - 1) * gridDim.x, stage == 0 ? p.depth - 1 : stage - 1);
+  for (int k = 0; k < p.depth - 1; ++k) in.ask(in.mine_of(in.first() + k * in.step()), k);
+  for (uint32_t set = in.first(); set < p.rows; set += in.step()) {
+    const uint32_t row = in.mine_of(set);
+    in.ask(row + (p.depth - 1) * in.step(), stage == 0 ? p.depth - 1 : stage - 1);
     if (turn == 0) {
-      const uint64_t mine = row + (uint64_t)in.lane * gridDim.x;
+      const uint64_t mine = row + (uint64_t)in.lane * in.step();
       if (mine < p.rows) {
         if (post) rhs = p.rstd_h[mine];
         if (in.has(kDn)) rys = p.rstd_y[mine];
@@ -363,9 +398,9 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
       }
     }
     constexpr unsigned kAll = 0xffffffffu;
-    const float rh = __shfl_sync(kAll, rhs, turn), ry = __shfl_sync(kAll, rys, turn),
-                gate = __shfl_sync(kAll, gates, turn);
-    turn = (turn + 1) & 31;
+    const float rh = __shfl_sync(kAll, rhs, turn, LANES), ry = __shfl_sync(kAll, rys, turn, LANES),
+                gate = __shfl_sync(kAll, gates, turn, LANES);
+    turn = (turn + 1) & (LANES - 1);
     if constexpr (MODE != kSingle) copy_async_wait(p.depth - 1);
     float2 hh[NG][4], yh[NG][4], t[NG][4];  // t = dy + ry u, so that Y = t - ry yh mean(u yh)
     // sums of u yh, and of c = e hh with t and yh
@@ -399,10 +434,10 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
         s2 = fma2(c[i], yh[g][i], s2);
       }
     }
-    const float3 s = cta_sum3(make_float3(s0.x + s0.y, s1.x + s1.y, s2.x + s2.y), red, par);
+    const float3 s = cta_sum3<LANES>(make_float3(s0.x + s0.y, s1.x + s1.y, s2.x + s2.y), red, par);
     const float rm = ry * s.x * inv_d;
     const float cy = s.y - rm * s.z;  // sum of c Y
-    if (p.gate_kind == kGateRow && p.dgate != nullptr && threadIdx.x == 0) static_cast<float*>(p.dgate)[row] = cy;
+    if (p.gate_kind == kGateRow && p.dgate != nullptr && in.leads(row)) static_cast<float*>(p.dgate)[row] = cy;
     // without a post norm rh is 1 and dh has no mean
     const float2 minus_rm = both(-rm), minus_k = both(post ? -rh * gate * cy * inv_d : 0.f), r = both(rh * gate);
 #pragma unroll
@@ -437,6 +472,18 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
   }
   if constexpr (MODE != kSingle) copy_async_wait(0);
   if (p.part == nullptr) return;
+  if constexpr (LANES < 32) {
+#pragma unroll
+    for (int o = 16; o >= LANES; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        for (float2* v : {&sum_pre[0][i], &sum_q[0][i]}) {
+          v->x += __shfl_xor_sync(0xffffffffu, v->x, o);
+          v->y += __shfl_xor_sync(0xffffffffu, v->y, o);
+        }
+      }
+    if ((threadIdx.x & 31) >= LANES) return;
+  }
   float* part = p.part + (int64_t)blockIdx.x * 2 * p.d;
 #pragma unroll
   for (int g = 0; g < NG; ++g)
@@ -479,7 +526,7 @@ __global__ void __launch_bounds__(kFinishWarps * 32)
 
 struct Shape {
   Mode mode;
-  int threads, groups, ins;
+  int threads, groups, ins, lanes;
 };
 
 // wide_from: 256-column groups in an aligned row from which a thread takes two of them.
@@ -495,7 +542,7 @@ Shape shape_of(const NormParams& p, int esize, int wide_from) {
   }
   for (const void* q : {p.y, p.n, p.dx, p.dh}) ok = ok && reinterpret_cast<uintptr_t>(q) % 16 == 0;
   if (p.gate_kind == kGateFull) ok = ok && reinterpret_cast<uintptr_t>(p.dgate) % 16 == 0;
-  Shape s{!ok ? kSingle : p.d % v == 0 ? kAligned : kShifted, 0, 0, ins};
+  Shape s{!ok ? kSingle : p.d % v == 0 ? kAligned : kShifted, 0, 0, ins, 32};
   const int per = (p.d + (s.mode == kShifted ? v - 1 : 0) + 255) / 256;
   s.groups = per >= (s.mode == kAligned ? wide_from : kWide) ? 2 : 1;
   s.threads = (per + s.groups - 1) / s.groups * 32;
@@ -504,24 +551,36 @@ Shape shape_of(const NormParams& p, int esize, int wide_from) {
     s.mode = kSingle;
     s.threads = std::min(s.threads, 1024);
   }
+  // Several short rows to a warp: 131072 x 64 bf16 11.8 and 16.5 us, with one each 34 and 50 us; x 128 23.5 and 38 us,
+  // with one each 34.5 and 51 us.
+  if (s.mode == kAligned && p.d <= 128) s.lanes = p.d <= 64 ? 8 : 16;
   return s;
 }
 
-// f(MODE, NG, ALL, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
+// f(MODE, NG, LANES, ALL, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
 template <typename F>
 void with_shape(const Shape& s, bool all, F&& f) {
   using std::integral_constant;
+  using One = integral_constant<int, 1>;
+  using Two = integral_constant<int, 2>;
+  using Warp = integral_constant<int, 32>;
   auto go = [&](auto mode, auto every) {
     if (s.groups == 2 && s.threads > 512)
-      f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 1024>{});
+      f(mode, Two{}, Warp{}, every, integral_constant<int, 1024>{});
     else if (s.groups == 2 && s.threads > 256)
-      f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 512>{});
+      f(mode, Two{}, Warp{}, every, integral_constant<int, 512>{});
     else if (s.groups == 2)
-      f(mode, integral_constant<int, 2>{}, every, integral_constant<int, 256>{});
+      f(mode, Two{}, Warp{}, every, integral_constant<int, 256>{});
     else if (s.threads > 256)
-      f(mode, integral_constant<int, 1>{}, every, integral_constant<int, 512>{});
-    else
-      f(mode, integral_constant<int, 1>{}, every, integral_constant<int, 256>{});
+      f(mode, One{}, Warp{}, every, integral_constant<int, 512>{});
+    else if (decltype(mode)::value != kAligned || s.lanes == 32)
+      f(mode, One{}, Warp{}, every, integral_constant<int, 256>{});
+    else if constexpr (decltype(mode)::value == kAligned) {
+      if (s.lanes == 16)
+        f(mode, One{}, integral_constant<int, 16>{}, every, integral_constant<int, 256>{});
+      else
+        f(mode, One{}, integral_constant<int, 8>{}, every, integral_constant<int, 256>{});
+    }
   };
   auto with = [&](auto mode) { all ? go(mode, std::true_type{}) : go(mode, std::false_type{}); };
   if (s.mode == kAligned)
@@ -534,7 +593,8 @@ void with_shape(const Shape& s, bool all, F&& f) {
 
 // The grid, with rows of a CTA that lie alike where that is needed.
 unsigned grid_of(int64_t wanted, const NormParams& p, const Shape& s, int esize) {
-  int64_t grid = std::min<int64_t>(p.rows, wanted);
+  const int per = 32 / s.lanes;  // rows at a time
+  int64_t grid = std::min<int64_t>((p.rows + per - 1) / per, wanted);
   const int v = 16 / esize;
   if (s.mode == kShifted && grid < p.rows) grid = std::min<int64_t>(p.rows, std::max<int64_t>(v, grid / v * v));
   return (unsigned)grid;
@@ -619,10 +679,11 @@ void residual_norm_fwd_launch(const ResidualNormArgs& a, const at::Tensor& y, co
     using T = decltype(t);
     const Shape s = shape_of(p, sizeof(T), kWide);
     const bool all = p.in[kH] != nullptr && p.n != nullptr && a.gate_kind != kGateFull;
-    with_shape(s, all, [&](auto mode, auto ng, auto every, auto maxt) {
+    with_shape(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 1024 ? 1 : 1024 / kMaxT;
       constexpr auto kernel =
-          residual_norm_fwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>;
+          residual_norm_fwd<T, decltype(mode)::value, decltype(ng)::value, decltype(lanes)::value,
+                            decltype(every)::value, kMaxT, kMinB>;
       const int64_t resident = plan_ring(p, s, sizeof(T), fit_of<kernel>(s.threads), 4);
       launch_norm(kernel, p, s, grid_of(resident, p, s, sizeof(T)));
     });
@@ -660,13 +721,14 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
     // an SM do better than 16 (16384 x 2048 bf16 71.4 us against 73.5 us, 4096 x 4096 40.3 us against 42 us). The kernel
     // for any set of inputs needs too many registers for that (8192 x 2048 with a gate per element 64 us against 57 us).
     const Shape s = shape_of(p, sizeof(T), all ? 5 : kWide);
-    with_shape(s, all, [&](auto mode, auto ng, auto every, auto maxt) {
+    with_shape(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = decltype(ng)::value == 1 && kMaxT == 256 ? 2 : 1;
       constexpr auto kernel =
-          residual_norm_bwd<T, decltype(mode)::value, decltype(ng)::value, decltype(every)::value, kMaxT, kMinB>;
+          residual_norm_bwd<T, decltype(mode)::value, decltype(ng)::value, decltype(lanes)::value,
+                            decltype(every)::value, kMaxT, kMinB>;
       int64_t grid = plan_ring(p, s, sizeof(T), fit_of<kernel>(s.threads), 4);
       // a few rows for each CTA at least: its partial sums cost as much as two rows
-      if (p.want_dpre || p.want_q) grid = std::min<int64_t>(grid, (p.rows + 3) / 4);
+      if (p.want_dpre || p.want_q) grid = std::min<int64_t>(grid, (p.rows * 1ll + 4 * 32 / s.lanes - 1) / (4 * 32 / s.lanes));
       grid = grid_of(grid, p, s, sizeof(T));
       at::Tensor part;
       if (p.want_dpre || p.want_q) {

@@ -435,6 +435,60 @@ def test_residual_norm_rows_off_16_bytes(dtype, rows, d, gate):
     _check_norm(t, dy, dn)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("rows,d", [(1, 8), (2, 40), (3, 64), (5, 48), (6, 128), (1, 128), (4097, 64), (2049, 72),
+                                    (20001, 64), (10001, 120)])
+@pytest.mark.parametrize("gate", ["none", "channel", "row", "full"])
+def test_residual_norm_short_rows(dtype, rows, d, gate):
+    t, dy, dn = _norm_case(rows, d, dtype, True, True, gate, 21)
+    _check_norm(t, dy, dn)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [3, 9, 601])
+def test_rms_norm_of_heads(rows, d):
+    """[tokens, heads, d] views of a packed matrix, which stays as it was."""
+    from mtorus.ops.residual_norm import rms_norm
+
+    g = _gen(22)
+    packed = torch.randn(rows, 5 * d, generator=g, device=DEV).to(BF)
+    kept = packed.clone()
+    w = torch.randn(d, generator=g, device=DEV)
+    for part in (packed[:, :d], packed[:, d:4 * d].unflatten(1, (3, d)), packed.unflatten(1, (5, d))):
+        x = part.detach().requires_grad_()
+        n = rms_norm(x, w.requires_grad_(), eps=1e-6)
+        dn = torch.randn(n.shape, generator=g, device=DEV).to(BF)
+        dx, dw = torch.autograd.grad(n, [x, w], dn)
+        flat = x.detach().reshape(-1, d)
+        ref = _ref_norm(flat, torch.zeros_like(flat), w, None, None, 1.0, 0.0, 1e-6, None, dn.reshape(-1, d))
+        _close(n.reshape(-1, d), *ref["n"], FWD_ROUNDINGS, "n")
+        _close(dx.reshape(-1, d), *ref["dx"], BWD_ROUNDINGS, "dx")
+        _close(dw, *ref["dpre"], COL_ROUNDINGS, "dw")
+    assert torch.equal(packed, kept)
+
+
+@pytest.mark.parametrize("d", [64, 120])
+def test_residual_norm_short_rows_do_not_mix(d):
+    """A row of NaN or infinity changes its own results only (and the column sums), whichever rows share its warp."""
+    from mtorus.ops.residual_norm import residual_norm
+
+    t, dy, dn = _norm_case(13, d, BF, True, True, "row", 23)
+
+    def run(t):
+        leaf = {k: v.detach().requires_grad_() for k, v in t.items()}
+        y, n = residual_norm(leaf["x"], leaf["h"], pre_weight=leaf["pre"], post_weight=leaf["post"], gate=leaf["gate"])
+        return [y, n, *torch.autograd.grad([y, n], [leaf["x"], leaf["h"], leaf["gate"]], [dy, dn])]
+
+    want = run(t)
+    for row, value in ((0, math.nan), (5, math.inf), (12, math.nan)):
+        x = t["x"].clone()
+        x[row] = value
+        others = [i for i in range(13) if i != row]
+        for a, b in zip(run(dict(t, x=x)), want):
+            assert torch.equal(a[others], b[others])
+            assert not torch.isfinite(a[row].float()).all()
+
+
 def test_residual_norm_rows_off_16_bytes_of_a_wider_matrix():
     """Rows of 257 values, 769 apart: what lies between them is neither used nor, in the outputs, written."""
     g = _gen(15)
