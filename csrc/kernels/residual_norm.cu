@@ -496,26 +496,31 @@ __global__ void __launch_bounds__(MAXT, MINB) residual_norm_bwd(const __grid_con
     }
 }
 
-// Sums the CTAs' parts in a fixed order, one CTA for 32 columns: dpre, or q and from it dpost = alpha g q and
-// dgate = alpha post q.
-constexpr int kFinishWarps = 32;
-__global__ void __launch_bounds__(kFinishWarps * 32)
+// Sums the CTAs' parts in a fixed order, one CTA for COLS columns: dpre, or q and from it dpost = alpha g q and
+// dgate = alpha post q. Bound by the latency of its loads: 8 columns to a CTA where there are few (131072 x 64 bf16
+// 5.1 us, with 32 10 us; 16727 x 1003 4.6 and 5.6 us), 32 for wide rows (16384 x 2048 4.5 us, with 8 6.7 us).
+constexpr int kFinishThreads = 1024;
+template <int COLS>
+__global__ void __launch_bounds__(kFinishThreads)
     residual_norm_finish(const float* part, int parts, int d, bool first, float alpha, const float* gate,
                          const float* post, float* dpre, float* dpost, float* dgate) {
-  __shared__ float sm[kFinishWarps][32];
+  constexpr int kWarps = kFinishThreads / 32;
+  __shared__ float sm[kWarps][COLS];
   const bool is_pre = first && blockIdx.y == 0;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * COLS + threadIdx.x % COLS;
   float t = 0.f;
   if (c < d) {
     const float* col = part + (is_pre ? 0 : d) + c;
 #pragma unroll 4
-    for (int b = w; b < parts; b += kFinishWarps) t += col[(int64_t)b * 2 * d];
+    for (int b = threadIdx.x / COLS; b < parts; b += kFinishThreads / COLS) t += col[(int64_t)b * 2 * d];
   }
-  sm[w][lane] = t;
-  __syncthreads();
-  if (w != 0 || c >= d) return;
 #pragma unroll
-  for (int k = 1; k < kFinishWarps; ++k) t += sm[k][lane];
+  for (int o = 16; o >= COLS; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (lane < COLS) sm[w][lane] = t;
+  __syncthreads();
+  if (threadIdx.x >= COLS || c >= d) return;
+#pragma unroll
+  for (int k = 1; k < kWarps; ++k) t += sm[k][lane];
   if (is_pre) {
     dpre[c] = t;
   } else {
@@ -737,10 +742,16 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
       }
       launch_norm(kernel, p, s, (unsigned)grid);
       if (p.part != nullptr) {
-        residual_norm_finish<<<dim3((p.d + 31) / 32, p.want_dpre + p.want_q), kFinishWarps * 32, 0, cur_stream()>>>(
-            p.part, (int)grid, p.d, p.want_dpre, p.alpha, a.gate_kind == kGateChannel ? p.gate : nullptr, p.post,
-            p.want_dpre ? dpre.data_ptr<float>() : nullptr, dpost.defined() ? dpost.data_ptr<float>() : nullptr,
-            gate_sum ? dgate.data_ptr<float>() : nullptr);
+        auto finish = [&](auto kernel, int cols) {
+          kernel<<<dim3((p.d + cols - 1) / cols, p.want_dpre + p.want_q), kFinishThreads, 0, cur_stream()>>>(
+              p.part, (int)grid, p.d, p.want_dpre, p.alpha, a.gate_kind == kGateChannel ? p.gate : nullptr, p.post,
+              p.want_dpre ? dpre.data_ptr<float>() : nullptr, dpost.defined() ? dpost.data_ptr<float>() : nullptr,
+              gate_sum ? dgate.data_ptr<float>() : nullptr);
+        };
+        if (p.d <= 1024)
+          finish(residual_norm_finish<8>, 8);
+        else
+          finish(residual_norm_finish<32>, 32);
         MT_LAUNCH_CHECK();
       }
     });
