@@ -534,9 +534,21 @@ struct Shape {
   int threads, groups, ins, lanes;
 };
 
-// wide_from: 256-column groups in an aligned row from which a thread takes two of them.
-constexpr int kWide = 17;  // more do not fit the registers of a CTA's threads otherwise
-Shape shape_of(const NormParams& p, int esize, int wide_from) {
+constexpr int kWide = 17;  // 256-column groups of a row; more do not fit the registers of a CTA's threads otherwise
+
+// Whether a thread of the backward for known inputs takes two groups of an aligned row. Its registers allow 8 warps on
+// an SM: with a barrier for every row, 8 warps that do more each beat 16 (16384 x 2048 bf16 71.4 us against 73.5 us,
+// 4096 x 4096 40.3 us against 42 us, 9362 x 1792 41.6 us against 43.2 us), but not where whole CTAs leave 2 or more of
+// the 8 empty (13107 x 1280 49.5 us against 41.6 us, 7281 x 2304 56 us against 52.5 us). In 32 bits they are as fast or
+// faster at every width, by up to 13 % (16256 x 1032 67 us against 78 us). The kernel for any set of inputs needs too
+// many registers for it (8192 x 2048 with a gate per element 64 us against 57 us).
+bool two_groups(int groups, int esize) {
+  const int warps = (groups + 1) / 2;
+  return groups >= 5 && (esize == 4 || 8 / warps * warps >= 7);
+}
+
+// pairs: two groups for a thread also where two_groups() says so.
+Shape shape_of(const NormParams& p, int esize, bool pairs) {
   const int v = 16 / esize;
   bool ok = true;
   int ins = 0;
@@ -549,7 +561,7 @@ Shape shape_of(const NormParams& p, int esize, int wide_from) {
   if (p.gate_kind == kGateFull) ok = ok && reinterpret_cast<uintptr_t>(p.dgate) % 16 == 0;
   Shape s{!ok ? kSingle : p.d % v == 0 ? kAligned : kShifted, 0, 0, ins, 32};
   const int per = (p.d + (s.mode == kShifted ? v - 1 : 0) + 255) / 256;
-  s.groups = per >= (s.mode == kAligned ? wide_from : kWide) ? 2 : 1;
+  s.groups = per >= kWide || (pairs && s.mode == kAligned && two_groups(per, esize)) ? 2 : 1;
   s.threads = (per + s.groups - 1) / s.groups * 32;
   // a row has to fit into the ring, and into a CTA
   if (s.mode != kSingle && (ins * s.groups * s.threads * 8 * esize > kSmemBudget || s.threads > 1024)) {
@@ -682,7 +694,7 @@ void residual_norm_fwd_launch(const ResidualNormArgs& a, const at::Tensor& y, co
   if (p.rows == 0) return;
   dispatch_act(a.x.scalar_type(), [&](auto t) {
     using T = decltype(t);
-    const Shape s = shape_of(p, sizeof(T), kWide);
+    const Shape s = shape_of(p, sizeof(T), false);
     const bool all = p.in[kH] != nullptr && p.n != nullptr && a.gate_kind != kGateFull;
     with_shape(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 1024 ? 1 : 1024 / kMaxT;
@@ -722,10 +734,7 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
     using T = decltype(t);
     bool all = a.gate_kind != kGateFull;
     for (const void* q : {p.in[kH], p.in[kDy], p.in[kDn], (const void*)p.dx, (const void*)p.dh}) all = all && q != nullptr;
-    // Two groups for a thread from d = 1025 on: with a barrier for every row, 4 warps that do more each and 8 of them on
-    // an SM do better than 16 (16384 x 2048 bf16 71.4 us against 73.5 us, 4096 x 4096 40.3 us against 42 us). The kernel
-    // for any set of inputs needs too many registers for that (8192 x 2048 with a gate per element 64 us against 57 us).
-    const Shape s = shape_of(p, sizeof(T), all ? 5 : kWide);
+    const Shape s = shape_of(p, sizeof(T), all);
     with_shape(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = decltype(ng)::value == 1 && kMaxT == 256 ? 2 : 1;
       constexpr auto kernel =
