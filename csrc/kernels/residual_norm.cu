@@ -8,8 +8,8 @@
 // and the weight gradients see the value before its rounding.
 //
 // Bound by memory: forward 2 reads and 2 writes of [T, d], backward 4 and 2.  One CTA of d / 8 threads (or
-// d / 16) walks a strided set of rows; a thread owns the same 8 (16) columns of every row, so the weights and the sums of weight
-// gradients stay in its registers.  Its vectors of the next rows are on their way through a ring in shared memory;
+// d / 16) walks a strided set of rows; a thread owns the same 8 (16) columns of every row, so the weights and the sums
+// of weight gradients stay in its registers.  Its vectors of the next rows are on their way through a ring in shared memory;
 // each thread reads back only what it copied itself, so the ring needs no barrier. Rows of up to 128 columns (the norm
 // of a head) share a warp.
 //
@@ -221,8 +221,8 @@ struct Rows {
   }
 };
 
-// Sum of one value over the CTA (LANES < 32: over the lanes of a row) for every thread. `red` holds [2][kMaxWarps] floats; `par` alternates between its
-// halves, so that one barrier per call is enough.
+// Sum of one value over the CTA (LANES < 32: over the lanes of a row) for every thread. `red` holds [2][kMaxWarps]
+// floats; `par` alternates between its halves, so that one barrier per call is enough.
 template <int LANES>
 __device__ __forceinline__ float cta_sum(float v, float* red, int& par) {
   if constexpr (LANES < 32) {
@@ -742,7 +742,10 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
                             decltype(every)::value, kMaxT, kMinB>;
       int64_t grid = plan_ring(p, s, sizeof(T), fit_of<kernel>(s.threads), 4);
       // a few rows for each CTA at least: its partial sums cost as much as two rows
-      if (p.want_dpre || p.want_q) grid = std::min<int64_t>(grid, (p.rows * 1ll + 4 * 32 / s.lanes - 1) / (4 * 32 / s.lanes));
+      if (p.want_dpre || p.want_q) {
+        const int64_t few = 4 * 32 / s.lanes;
+        grid = std::min<int64_t>(grid, (p.rows + few - 1) / few);
+      }
       grid = grid_of(grid, p, s, sizeof(T));
       at::Tensor part;
       if (p.want_dpre || p.want_q) {
