@@ -144,7 +144,9 @@ __device__ __forceinline__ float largest(const Vec<T, 16 / sizeof(T)> (&v)[N]) {
 // the first has to rescale the sums (a warp does when one of its lanes does). r is rounded; that shifts all exponents
 // alike and fast_done() takes it out again. For the weighted sum, values are kept at -1e30 or above (fp16: at its
 // lowest), so that an exponent is finite and a masked value adds 0 * finite. Good for maxima from -2^26 / c to
-// 2^26 / c that lie well above that; fast_done() says so.
+// 2^26 / c that lie well above that; fast_done() says so. No value may lie above the reference by more than the slack,
+// the lifted ones that come before any other among them: so the reference starts at -2^26 / c, or, where it is higher, at
+// the value that masked ones are lifted to (1 each, until the first possible value scales them away).
 struct Fast {
   float m, minus_r, limit, best;  // limit: the maximum up to which m stays; best: the maximum
   float2 s, w;
@@ -153,8 +155,17 @@ struct Fast {
 constexpr float kFastLimit = 67108864.f;  // 2^26: r is rounded by at most 2
 constexpr float kSlack = 8.f;
 
+template <typename T>
+__device__ __forceinline__ constexpr float kept_above() {
+  return std::is_same_v<T, __half> ? -65504.f : -1e30f;
+}
+
+template <typename T, bool ENT>
 __device__ __forceinline__ Fast fast_start(float c) {
-  return Fast{-kFastLimit / c, kFastLimit, -kFastLimit / c, -INFINITY, both(0.f), both(0.f)};
+  const float least = -kFastLimit / c;
+  const bool lifted = ENT && kept_above<T>() > least;
+  const float m = lifted ? kept_above<T>() : least;
+  return Fast{m, lifted ? -(m * c) : kFastLimit, m, -INFINITY, both(0.f), both(0.f)};
 }
 
 template <bool ENT>
@@ -165,11 +176,6 @@ __device__ __forceinline__ void fast_raise(Fast& a, float vm, float c) {
   a.m = vm;
   a.minus_r = minus_r;
   a.limit = vm + kSlack / c;
-}
-
-template <typename T>
-__device__ __forceinline__ constexpr float kept_above() {
-  return std::is_same_v<T, __half> ? -65504.f : -1e30f;
 }
 
 template <typename T, bool ENT>
@@ -205,7 +211,7 @@ __device__ __forceinline__ bool fast_done(const Fast& a, float c, Running& out) 
     return true;
   }
   if (a.best == -INFINITY) return true;  // nothing, or masked values only
-  if (a.best < a.m) return false;        // below the lower limit
+  if (a.best < a.m) return false;        // below the start
   if (ENT && (kept_above<T>() - a.m) * c > -200.f) return false;
   const float d = fmaf(a.m, c, a.minus_r), f = ex2(-d);
   out = Running{a.m, s * f, f * fmaf(-d, s, w)};
@@ -552,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, NT == 32 ? 4 : TOP == kTopHere ? 2 :
 
   // one pass, a tile after the other
   const int64_t tiles = (parts.vectors + TILE - 1) / TILE;
-  Fast sums = fast_start(p.c);
+  Fast sums = fast_start<T, ENT>(p.c);
   auto take = [&](const auto& v) {  // the values of one or more vectors; their maximum
     const float vm = largest<T>(v);
     sums.best = fmaxf(sums.best, vm);

@@ -1,0 +1,64 @@
+"""More of the decoder operators' edges on the GPU, against the plain 64-bit forms and bounds of
+``test_decoder_ops_gpu``: sparse masks in every type."""
+import pytest
+import test_decoder_ops_gpu as ops
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda"
+
+
+# ------------------------------------------------------------------------- masked logits before possible ones
+
+
+def _masked(rows, V, dtype, mask, seed):
+    """Logits of which ``mask`` leaves a part, each row's token among them."""
+    x, _ = ops._logits(rows, V, dtype, seed)
+    g = ops._gen(seed + 1)
+    if mask == "leading":
+        keep = torch.arange(V, device=DEV).expand(rows, V) >= (V * 2) // 5
+    elif mask == "all but the last":
+        keep = torch.arange(V, device=DEV).expand(rows, V) >= V - 5
+    else:  # one in a thousand, and the last so that none is empty
+        keep = torch.rand(rows, V, generator=g, device=DEV) < 1e-3
+        keep[:, -1] = True
+    t = torch.multinomial(keep.float(), 1, generator=g)[:, 0]
+    return x.masked_fill(~keep, float("-inf")), t
+
+
+@pytest.mark.parametrize("dtype", [HF, BF, F32])
+@pytest.mark.parametrize("mask", ["leading", "all but the last", "sparse"])
+@pytest.mark.parametrize("rows,V", [(3, 50000), (400, 50001), (5, 3000), (400, 2048), (401, 301)])
+def test_logprobs_masked_before_possible(rows, V, mask, dtype):
+    """Whole tiles, vectors and threads without a possible token, before or between the possible ones."""
+    x, t = _masked(rows, V, dtype, mask, 30)
+    # the temperatures put the exponents' range on both sides of fp16's lowest value; the least of them for the
+    # smaller cases only
+    for tau in (1.0, 0.05) if rows * V > 10 ** 7 else (1.0, 0.05, 1e-4, 30.0, 2000.0):
+        r = ops._check_logprobs(x, t, tau=tau, top=4)
+        assert torch.isfinite(r.logprob).all() and torch.isfinite(r.entropy).all()
+    ops._check_logprobs(x, t, top=4, entropy=False)
+
+
+@pytest.mark.parametrize("V", [5, 40, 301, 2048, 4099])
+def test_logprobs_many_short_rows_fp16(V):
+    ops.test_logprobs_many_short_rows(HF, V)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_logprobs_nan_and_inf_stay_in_their_row_fp16(bad):
+    ops.test_logprobs_nan_and_inf_stay_in_their_row(bad, HF)
+
+
+@pytest.mark.parametrize("V", [3000, 70000])
+def test_logprobs_rise_over_the_whole_range_fp16(V):
+    """Each thread's maximum rises from fp16's lowest value to its largest, with masked values between."""
+    i = torch.arange(V, device=DEV).double()
+    x = torch.stack([-65504 + 131008 * i / (V - 1), 65504 * i / (V - 1), -65504 + i / V, i * 0 + 65504]).to(HF)
+    x[:, 1::3] = float("-inf")
+    t = torch.tensor([V - 1 - (V - 1) % 3, 0, 3, 6], device=DEV)
+    for tau in (1.0, 1e-3, 1e3):
+        for ent in (True, False):
+            ops._check_logprobs(x, t, tau=tau, top=4, entropy=ent)
