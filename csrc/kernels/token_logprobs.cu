@@ -692,10 +692,17 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd(const __grid_cons
   const float gh = ENT ? p.g_entropy[row] * p.inv_tau : 0.f;
   const float h = ENT ? p.entropy[row] : 0.f;
   float total = gl;
+  bool any = use || gh != 0.f;
   if (p.g_top != nullptr) {
-    for (int i = 0; i < p.top; ++i) total += p.g_top[row * p.top + i] * p.inv_tau;
+    for (int i = 0; i < p.top; ++i) {
+      const float g = p.g_top[row * p.top + i];
+      any = any || g != 0.f;
+      total += g * p.inv_tau;
+    }
   }
-  const bool none = l2s == -INFINITY;  // no possible token: no gradient
+  // No gradient: no possible token, or an ignored one and nothing else comes in (then the logits may be anything, such as
+  // NaN in the rows that pad a batch).
+  const bool none = l2s == -INFINITY || !any;
   auto grad = [&](float v) {
     const float t = max_nan(fmaf(v - m, p.c, -l2s), -200.f);  // log2 of the probability
     const float e = ex2(t);

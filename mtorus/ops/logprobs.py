@@ -14,12 +14,13 @@ Logits are bf16, fp16 or fp32 [..., V] (any row stride; rows that are not dense 
 copied first), tokens int64 [...], top at most 64 and at most V.  Sums are held in fp32.
 
 * A token outside [0, V) is ignored: its logprob is 0 and has no gradient.  Entropy and
-  alternatives of its row are computed all the same.
+  alternatives of its row are computed all the same; where their gradients are absent or 0, the
+  row's gradient is 0 whatever its logits are.
 * Masked logits (-inf, or the type's lowest value) have probability 0 unless the whole row is at
   that value.  A row of -inf only: logprob -inf, entropy 0, no gradient.
 * Alternatives order by value, equal values by the lowest id.  Where fewer than ``top`` tokens are
   possible, impossible ones follow with logprob -inf.
-* A row with a NaN or +inf has NaN results and gradients (its ids rank NaN with -inf).
+* Otherwise a row with a NaN or +inf has NaN results and gradients (its ids rank NaN with -inf).
 
 A CUDA graph that records the backward must be the only holder of an autograd
 graph of its leaves: drop eager results of the same leaves before the capture.

@@ -1,5 +1,5 @@
 """More of the decoder operators' edges on the GPU, against the plain 64-bit forms and bounds of
-``test_decoder_ops_gpu``: sparse masks in every type."""
+``test_decoder_ops_gpu``: sparse masks in every type, padded batches."""
 import pytest
 import test_decoder_ops_gpu as ops
 import torch
@@ -62,3 +62,40 @@ def test_logprobs_rise_over_the_whole_range_fp16(V):
     for tau in (1.0, 1e-3, 1e3):
         for ent in (True, False):
             ops._check_logprobs(x, t, tau=tau, top=4, entropy=ent)
+
+
+# -------------------------------------------------------------------------------------------- padded batches
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,V", [(6, 513), (6, 50257), (400, 1003)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_logprobs_padded_rows_have_no_gradient(bad, rows, V, dtype):
+    """Rows behind the last sequence: whatever their logits hold, an ignored token brings no gradient into them, nor do
+    zeros from the entropy and the alternatives."""
+    from mtorus.ops.logprobs import token_logprobs
+
+    x, t = ops._logits(rows, V, dtype, 40)
+    clean = x.clone()
+    pad = [1, rows - 1]
+    x[pad[0]] = bad
+    x[pad[1], V // 2:] = bad
+    t[pad] = -100
+    up = torch.randn(rows, generator=ops._gen(41), device=DEV)
+    up_pad = up.index_fill(0, torch.tensor(pad, device=DEV), 0.0)
+    grads = []
+    for src in (x, clean):
+        leaf = src.detach().requires_grad_()
+        r = token_logprobs(leaf, t, top=3, entropy=True)
+        assert (r.logprob[pad] == 0).all()
+        d = [torch.autograd.grad(r.logprob, leaf, up, retain_graph=True)[0],
+             torch.autograd.grad([r.logprob, r.entropy, r.top_logprobs], leaf,
+                                 [up, up_pad, up_pad[:, None].expand(rows, 3)], retain_graph=True)[0]]
+        if src is x:  # a gradient that does come into such a row is as undefined as its logits
+            (own,) = torch.autograd.grad(r.entropy, leaf, up)
+            assert torch.isnan(own[pad]).all()
+        grads.append(d)
+    for got, want in zip(*grads):
+        assert (got[pad] == 0).all()
+        others = [i for i in range(rows) if i not in pad]
+        assert torch.equal(got[others], want[others])
