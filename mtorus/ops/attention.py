@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 import torch
 
 from .._ext import cuda as _cuda
-from .rotary import RotaryPositions, rotary_, rotary_qkv
+from .rotary import RotaryPositions, rotary_gradient_, rotary_qkv
 
 HEAD_DIM = 128
 TILE = 128
@@ -85,7 +85,7 @@ class CausalAttentionFn(torch.autograd.Function):
         dqkv = attention_bwd(dout, qkv, out, lse, B, S, H)
         if ctx.rope is not None:  # dq and dk turn back where they lie
             heads = dqkv.view(B, S, 3 * H, HEAD_DIM)
-            rotary_(heads[:, :, :H], heads[:, :, H:2 * H], ctx.rope, positions, inverse=True)
+            rotary_gradient_(heads[:, :, :H], heads[:, :, H:2 * H], ctx.rope, positions)
         return dqkv, None, None, None, None, None
 
 

@@ -125,8 +125,21 @@ def rotary_qkv(qkv: torch.Tensor, B: int, S: int, H: int, rope: RotaryPositions,
 def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], rope: RotaryPositions,
             positions: Optional[torch.Tensor] = None, *, offset: int = 0, inverse: bool = False) -> None:
     """Rotates q and k where they lie (views of a cache or of a packed matrix included: any strides
-    with a dense head dim), by minus the angle with ``inverse``.  Records no gradient and refuses
-    tensors that require one; values outside the rotated heads are not touched.  q and k must not
-    share memory."""
+    with a dense head dim); ``inverse`` undoes that: minus the angle, divided by the attention scale.
+    Records no gradient and refuses tensors that require one; values outside the rotated heads are
+    not touched.  q and k must not share memory."""
     rope._check(q.shape[-1])
-    _cuda().rotary_inplace(q, k, *rope.args, positions, offset, inverse)
+    scale = rope.scale
+    if inverse:
+        if scale == 0.0:
+            raise ValueError("rotary_: an attention scale of 0 cannot be undone")
+        scale = 1.0 / scale
+    _cuda().rotary_inplace(q, k, *rope.args[:3], scale, positions, offset, inverse)
+
+
+def rotary_gradient_(dq: torch.Tensor, dk: torch.Tensor, rope: RotaryPositions,
+                     positions: Optional[torch.Tensor] = None, *, offset: int = 0) -> None:
+    """Turns the gradients of rotated q and k, where they lie, into those of q and k: minus the angle,
+    times the attention scale (the transpose of the rotation, where ``rotary_``'s inverse undoes it)."""
+    rope._check(dq.shape[-1])
+    _cuda().rotary_inplace(dq, dk, *rope.args, positions, offset, True)

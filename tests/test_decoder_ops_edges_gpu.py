@@ -1,5 +1,5 @@
 """More of the decoder operators' edges on the GPU, against the plain 64-bit forms and bounds of
-``test_decoder_ops_gpu``: sparse masks in every type, padded batches."""
+``test_decoder_ops_gpu``: sparse masks in every type, padded batches, rotary undone."""
 import pytest
 import test_decoder_ops_gpu as ops
 import torch
@@ -99,3 +99,50 @@ def test_logprobs_padded_rows_have_no_gradient(bad, rows, V, dtype):
         assert (got[pad] == 0).all()
         others = [i for i in range(rows) if i not in pad]
         assert torch.equal(got[others], want[others])
+
+
+# ------------------------------------------------------------------------------------- rotary there and back
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(scaling="yarn", factor=8.0), dict(attention_scale=-0.25)])
+def test_rotary_inverse_undoes(kw):
+    """Positions taken back and given anew, as for a cache that moves: fp32, so that only the arithmetic shows."""
+    from mtorus.ops.rotary import rotary_
+
+    rope = ops._rope(64, rot_dim=48, **kw)
+    g = ops._gen(50)
+    q = torch.randn(5, 3, 64, generator=g, device=DEV)
+    k = torch.randn(5, 2, 64, generator=g, device=DEV)
+    pos = torch.randint(0, 100000, (5,), generator=g, device=DEV)
+    for x, other in ((q, k), (k, None)):
+        a, b = x.clone(), None if other is None else other.clone()
+        rotary_(a, b, rope, pos)
+        rotary_(a, b, rope, pos, inverse=True)
+        for got, want in ((a, x), (b, other)):
+            if want is None:
+                continue
+            # each way rounds below 8 U of the pair's sum of absolute values (at most doubled by the way before it), and
+            # the scale and its reciprocal are rounded once each
+            half = want[..., :48].double().abs().unflatten(-1, (2, 24)).sum(-2).repeat(1, 1, 2)
+            off = (got[..., :48].double() - want[..., :48].double()).abs()
+            assert (off <= (3 * ops.ROT_ROUNDINGS + 2) * ops.U * half).all()
+            assert torch.equal(got[..., 48:], want[..., 48:])
+
+
+def test_causal_attention_gradient_with_scaled_rotary():
+    """The gradient of the turn is the turn back, times the attention scale (not divided by it)."""
+    from mtorus.ops.attention import causal_attention
+    from mtorus.ops.rotary import rotary_qkv
+
+    B, S, H = 1, 256, 2
+    g = ops._gen(51)
+    qkv = torch.randn(B * S, 3 * H * 128, generator=g, device=DEV).to(BF)
+    dout = torch.randn(B * S, H * 128, generator=g, device=DEV).to(BF)
+    rope = ops._rope(128, scaling="yarn", factor=16.0, original_len=64)
+    a, b = (qkv.clone().requires_grad_() for _ in range(2))
+    oa = causal_attention(a, B, S, H, 128, rotary=rope)
+    ob = causal_attention(rotary_qkv(b, B, S, H, rope), B, S, H, 128)
+    assert torch.equal(oa, ob)
+    (ga,), (gb,) = torch.autograd.grad(oa, a, dout), torch.autograd.grad(ob, b, dout)
+    # dQ's reduce-adds may come in another order: bf16 values of one fp32 sum, at most one step apart, then rotated
+    assert ((ga.double() - gb.double()).norm() / gb.double().norm()).item() <= 2.0 ** -7
