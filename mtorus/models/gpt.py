@@ -308,15 +308,17 @@ class GptModel(nn.Module):
             blk._qkv_b = _ParamView([a.q_proj.bias, a.k_proj.bias, a.v_proj.bias], self.flat, (3 * d,))
         return self.flat
 
-    def fused_hidden(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def fused_hidden(self, input_ids: torch.Tensor, plain: bool = False) -> torch.Tensor:
+        """plain: in bf16 and without dropout, whatever the model's training has switched on (its
+        FP8 and dropout states are neither used nor changed)."""
         from ..ops.fused import LayerNormFn
 
         assert self.flat is not None, "call flatten(device) before using the fused path"
         B, S = input_ids.shape
-        x = self.fused_blocks(self.fused_embed(input_ids), B, S)
+        x = self.fused_blocks(self.fused_embed(input_ids, plain), B, S, plain)
         return LayerNormFn.apply(x, (self.ln_f.gamma, self.ln_f.beta), self.ln_f.eps)
 
-    def fused_embed(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def fused_embed(self, input_ids: torch.Tensor, plain: bool = False) -> torch.Tensor:
         """[B, S] token ids -> [B*S, d] bf16 hidden (token + learned position embedding,
         then the embedding dropout when enabled)."""
         from ..ops.dropout import SITE_EMBED
@@ -324,7 +326,7 @@ class GptModel(nn.Module):
 
         assert self.flat is not None, "call flatten(device) before using the fused path"
         S = input_ids.shape[1]
-        ds = self.dropout_state
+        ds = None if plain else self.dropout_state
         return EmbeddingFn.apply(input_ids, grad_anchor(input_ids.device),
                                  (self.token_embedding.weight, self.position_embedding.weight), S,
                                  None if ds is None else ds.args(SITE_EMBED))
@@ -346,12 +348,12 @@ class GptModel(nn.Module):
         ds = self.dropout_state
         return None if ds is None else (ds, self.layer_offset + i)
 
-    def fused_blocks(self, x: torch.Tensor, B: int, S: int) -> torch.Tensor:
+    def fused_blocks(self, x: torch.Tensor, B: int, S: int, plain: bool = False) -> torch.Tensor:
         """[B*S, d] -> [B*S, d] through this model's (or stage's) transformer blocks."""
-        st = getattr(self, "fp8_state", None)
+        st = None if plain else getattr(self, "fp8_state", None)
         for i, blk in enumerate(self.blocks):
             x = blk.fused_forward(x, B, S, None if st is None else (st, f"L{self.layer_offset + i}"),
-                                  self._layer_drop(i))
+                                  None if plain else self._layer_drop(i))
         return x
 
     def fused_stage(self, x: torch.Tensor, B: int, S: int) -> torch.Tensor:
@@ -454,16 +456,11 @@ class GptModel(nn.Module):
         probability of its target (a target outside the vocabulary is ignored), and on request
         the entropy and the ``top`` likeliest tokens (``mtorus.ops.logprobs.TokenLogprobs``,
         [B, S] each).  Runs in bf16, without dropout, and records no gradient; FP8 scaling
-        histories and dropout keys of a training in progress stay as they are."""
+        histories and dropout keys of a training in progress are left alone."""
         from ..ops import kernels as K
         from ..ops.logprobs import token_logprobs
 
-        drop, fp8 = self.dropout_state, getattr(self, "fp8_state", None)
-        self.dropout_state = self.fp8_state = None
-        try:
-            h = self.fused_hidden(input_ids)
-        finally:
-            self.dropout_state, self.fp8_state = drop, fp8
+        h = self.fused_hidden(input_ids, plain=True)
         logits = K.gemm(h, self.lm_head.weight.w16, bias=self.lm_head.bias.data)
         return token_logprobs(logits.view(*targets.shape, self.vocab_size), targets, temperature=temperature, top=top,
                               entropy=entropy)
