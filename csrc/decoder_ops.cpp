@@ -6,9 +6,13 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <numeric>
 #include <tuple>
+#include <utility>
+#include <vector>
 
 #include "kernels/decoder_ops.h"
 
@@ -184,22 +188,77 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
   }
 };
 
-// Whether a token's heads of q and of k lie over one another, as two views of a packed matrix may. (Views that are not
-// dense as a whole are beyond at::assert_no_overlap.)
-bool share_heads(const at::Tensor& q, const at::Tensor& k) {
-  const int64_t n = q.dim(), D = q.size(-1), step = q.stride(-2);
-  if (q.numel() == 0 || k.numel() == 0 || !q.is_alias_of(k) || (k.size(-2) > 1 && q.size(-2) > 1 && k.stride(-2) != step))
-    return false;
-  for (int64_t i = 0; i < n - 2; ++i) {
-    if (q.size(i) > 1 && q.stride(i) != k.stride(i)) return false;
+// A multiple of `step` from `low` to `high`.
+struct Term {
+  int64_t step, low, high;
+};
+
+// Whether `at` plus a multiple of each term's step (falling) can come within `width` of 0. Exact, but for a layout so
+// entangled that `budget` trials do not settle it: true.
+bool can_meet(const std::vector<Term>& terms, size_t next, int64_t at, int64_t width, int& budget) {
+  if (next == terms.size()) return std::abs(at) < width;
+  if (--budget < 0) return true;
+  const Term& t = terms[next];
+  int64_t least = 0, most = 0;  // what the terms behind this one can add
+  int64_t grid = t.step;        // all that can be added is a multiple of this
+  for (size_t i = next + 1; i < terms.size(); ++i) {
+    least += terms[i].step * terms[i].low;
+    most += terms[i].step * terms[i].high;
+    grid = std::gcd(grid, terms[i].step);
   }
-  const int64_t between = k.storage_offset() - q.storage_offset();
-  const int64_t stride = q.size(-2) > 1 ? step : k.size(-2) > 1 ? k.stride(-2) : D;
-  // head j of k starts (between + (j - i) stride) values after head i of q
-  for (int64_t m = 1 - q.size(-2); m < k.size(-2); ++m) {
-    if (std::abs(between + m * stride) < D) return true;
+  const int64_t off = std::abs(at) % grid;
+  if (std::min(off, grid - off) >= width) return false;
+  auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t from = std::max(t.low, -floor_div(at + most + width - 1, t.step)),
+                to = std::min(t.high, floor_div(width - 1 - at - least, t.step));
+  for (int64_t m = from; m <= to; ++m) {
+    if (can_meet(terms, next + 1, at + m * t.step, width, budget)) return true;
   }
   return false;
+}
+
+// Whether heads of q and of k lie over one another, the same token's or different ones', as views of one buffer may. (Views
+// that are not dense as a whole are beyond at::assert_no_overlap.)
+bool share_heads(const at::Tensor& q, const at::Tensor& k) {
+  if (q.numel() == 0 || k.numel() == 0) return false;
+  const int64_t size = q.element_size(), width = q.size(-1) * size;
+  auto extent = [&](const at::Tensor& t) {
+    int64_t e = width;
+    for (int64_t i = 0; i < t.dim() - 1; ++i) e += (t.size(i) - 1) * t.stride(i) * size;
+    return e;
+  };
+  const int64_t between = reinterpret_cast<intptr_t>(k.data_ptr()) - reinterpret_cast<intptr_t>(q.data_ptr());
+  if (between >= extent(q) || -between >= extent(k)) return false;
+  // a head of k lies `between` + its own steps - those of the head of q from that
+  std::vector<Term> terms;
+  for (int sign : {-1, 1}) {
+    const at::Tensor& t = sign < 0 ? q : k;
+    for (int64_t i = 0; i < t.dim() - 1; ++i) {
+      if (t.size(i) == 1) continue;
+      const int64_t step = t.stride(i) * size, n = t.size(i) - 1;
+      auto same = std::find_if(terms.begin(), terms.end(), [&](const Term& o) { return o.step == step; });
+      if (same == terms.end()) same = terms.insert(same, Term{step, 0, 0});
+      (sign < 0 ? same->low : same->high) += sign * n;
+    }
+  }
+  std::sort(terms.begin(), terms.end(), [](const Term& a, const Term& b) { return a.step > b.step; });
+  int budget = 10000;
+  return can_meet(terms, 0, between, width, budget);
+}
+
+// Whether the heads of x are known to lie apart from one another: each axis steps over all that the smaller ones cover.
+bool heads_apart(const at::Tensor& x) {
+  std::vector<std::pair<int64_t, int64_t>> axes;
+  for (int64_t i = 0; i < x.dim(); ++i) {
+    if (x.size(i) > 1) axes.emplace_back(x.stride(i), x.size(i));
+  }
+  std::sort(axes.begin(), axes.end());
+  int64_t covered = 1;
+  for (const auto& [step, n] : axes) {
+    if (step < covered) return false;
+    covered += (n - 1) * step;
+  }
+  return true;
 }
 
 }  // namespace
@@ -256,12 +315,16 @@ void rotary_inplace(at::Tensor q, const OptTensor& k, const at::Tensor& turns, i
                 "rotary_: works in place and records no gradient; use rotary() on tensors that require one");
     TORCH_CHECK_VALUE(t->size(-1) <= 1 || t->stride(-1) == 1, "rotary_: the head dim must have stride 1");
     at::assert_no_internal_overlap(*t);
+    TORCH_CHECK_VALUE(t->numel() == 0 || heads_apart(*t), "rotary_: ", t == &q ? "q" : "k",
+                      " has heads that are the same memory in some of their values (sizes ", t->sizes(), ", strides ",
+                      t->strides(), ")");
   }
   if (kt.defined()) {
     check_pair(q, kt);
     TORCH_CHECK_VALUE(q.data_ptr() != kt.data_ptr() || q.numel() == 0, "rotary_: q and k are the same memory");
     at::assert_no_overlap(q, kt);
-    TORCH_CHECK_VALUE(!share_heads(q, kt), "rotary_: q and k are the same memory in some of their heads");
+    TORCH_CHECK_VALUE(!share_heads(q, kt), "rotary_: q and k are the same memory in some of their heads, or in a layout ",
+                      "too entangled to tell (strides ", q.strides(), " and ", kt.strides(), ")");
   }
   const at::Tensor qt = tokens_of(q);
   const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1));
