@@ -96,8 +96,9 @@ struct RotarySetup {
 // [.., H, D] -> [B, S, H, D]
 at::Tensor tokens_of(const at::Tensor& x) { return x.dim() == 3 ? x.unsqueeze(0) : x; }
 
-OptTensor positions_of(const OptTensor& positions, int64_t B, int64_t S) {
+OptTensor positions_of(const OptTensor& positions, int64_t B, int64_t S, int64_t offset) {
   if (!positions.has_value()) return c10::nullopt;
+  TORCH_CHECK_VALUE(offset == 0, "rotary: an offset (", offset, ") goes with the default positions only");
   const at::Tensor& p = *positions;
   TORCH_CHECK_TYPE(p.scalar_type() == at::kLong || p.scalar_type() == at::kInt,
                    "rotary: positions must be int64 or int32, not ", p.scalar_type());
@@ -273,7 +274,7 @@ std::tuple<at::Tensor, OptTensor> rotary(const at::Tensor& q, const OptTensor& k
     check_pair(q, *k);
   }
   const at::Tensor qt = tokens_of(q), kt = or_undefined(k);
-  const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1));
+  const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1), offset);
   check_cuda({&q, &kt, &turns, pos.has_value() ? &*pos : &turns}, "rotary");
   variable_list out;
   if (needs_grad({&q, &kt}))
@@ -296,7 +297,7 @@ at::Tensor rotary_qkv(const at::Tensor& qkv, int64_t B, int64_t S, int64_t heads
                     (heads + 2 * kv_heads) * head_dim, "], not ", qkv.sizes());
   const at::Tensor x = last_dense(qkv).unflatten(1, {heads + 2 * kv_heads, head_dim}).unflatten(0, {B, S});
   check_rotary(x, "qkv", r);
-  const OptTensor pos = positions_of(positions, B, S);
+  const OptTensor pos = positions_of(positions, B, S, offset);
   check_cuda({&qkv, &turns, pos.has_value() ? &*pos : &turns}, "rotary_qkv");
   const auto out = needs_grad({&x}) ? RotaryFn::apply(x, OptTensor(), turns, pos, rot_dim, interleaved, scale, offset,
                                                       heads + kv_heads)
@@ -327,7 +328,7 @@ void rotary_inplace(at::Tensor q, const OptTensor& k, const at::Tensor& turns, i
                       "too entangled to tell (strides ", q.strides(), " and ", kt.strides(), ")");
   }
   const at::Tensor qt = tokens_of(q);
-  const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1));
+  const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1), offset);
   check_cuda({&q, &kt, &turns, pos.has_value() ? &*pos : &turns}, "rotary_");
   c10::cuda::CUDAGuard guard(q.device());
   std::vector<RotarySegment> segs{{qt, qt, qt.size(2)}};

@@ -17,7 +17,8 @@ Tensors are bf16, fp16 or fp32, [tokens, heads, dim] or [batch, tokens, heads, d
 with any strides (rows that are not dense in the head dim are copied first), head
 dim at most 512; results are computed in fp32 and rounded once.  ``positions`` is
 int64 or int32, [tokens], [batch, tokens] or [1, tokens] ([batch] too, for one token
-per sequence); without it token i of a sequence has position ``offset + i``.
+per sequence); without it token i of a sequence has position ``offset + i`` (both
+together are refused).
 Positions are read on the device and may be any integer, negative ones included; an
 angle is as exact as its frequency in 64 bits (2^-53 of it).
 

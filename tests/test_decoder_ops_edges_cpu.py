@@ -4,7 +4,7 @@ import random
 import pytest
 import torch
 
-from mtorus.ops.rotary import RotaryPositions, rotary_
+from mtorus.ops.rotary import RotaryPositions, rotary, rotary_, rotary_qkv
 
 BF = torch.bfloat16
 
@@ -19,6 +19,17 @@ def test_rotary_inverse_of_a_zero_scale_is_refused():
         rotary_(q, None, _rope(attention_scale=0.0), inverse=True)
     with pytest.raises(RuntimeError, match="CUDA"):
         rotary_(q, None, _rope(attention_scale=0.0))
+
+
+def test_rotary_offset_with_positions_is_refused():
+    q, pos = torch.zeros(5, 4, 64, dtype=BF), torch.arange(5)
+    for call in (lambda **kw: rotary(q, None, _rope(), **kw), lambda **kw: rotary_(q, None, _rope(), **kw),
+                 lambda **kw: rotary_qkv(q.view(5, 256), 1, 5, 2, _rope(), kv_heads=1, **kw)):
+        with pytest.raises(ValueError, match="offset"):
+            call(positions=pos, offset=3)
+        for kw in (dict(positions=pos), dict(offset=3)):
+            with pytest.raises(RuntimeError, match="CUDA"):
+                call(**kw)
 
 
 # ------------------------------------------------------------------------------------------- scoring a model
