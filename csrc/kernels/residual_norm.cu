@@ -575,29 +575,30 @@ Shape shape_of(const NormParams& p, int esize, bool pairs) {
 }
 
 // f(MODE, NG, LANES, ALL, MAXT): the kernel for CTAs of up to MAXT threads, so that small ones get more registers.
-template <typename F>
+// PAIRS: shape_of()'s `pairs` where `all`. Without it two groups mean 9 warps at least, and so a MAXT above 256; with it a
+// thread never has one group of a row that takes 9 warps in 32 bits. Kernels that no shape asks for are not built.
+template <int ESIZE, bool PAIRS, typename F>
 void with_shape(const Shape& s, bool all, F&& f) {
   using std::integral_constant;
   using One = integral_constant<int, 1>;
   using Two = integral_constant<int, 2>;
   using Warp = integral_constant<int, 32>;
   auto go = [&](auto mode, auto every) {
-    if (s.groups == 2 && s.threads > 512)
-      f(mode, Two{}, Warp{}, every, integral_constant<int, 1024>{});
-    else if (s.groups == 2 && s.threads > 256)
-      f(mode, Two{}, Warp{}, every, integral_constant<int, 512>{});
-    else if (s.groups == 2)
-      f(mode, Two{}, Warp{}, every, integral_constant<int, 256>{});
-    else if (s.threads > 256)
-      f(mode, One{}, Warp{}, every, integral_constant<int, 512>{});
-    else if (decltype(mode)::value != kAligned || s.lanes == 32)
-      f(mode, One{}, Warp{}, every, integral_constant<int, 256>{});
-    else if constexpr (decltype(mode)::value == kAligned) {
-      if (s.lanes == 16)
-        f(mode, One{}, integral_constant<int, 16>{}, every, integral_constant<int, 256>{});
-      else
-        f(mode, One{}, integral_constant<int, 8>{}, every, integral_constant<int, 256>{});
+    constexpr bool kAl = decltype(mode)::value == kAligned, kPairs = PAIRS && kAl && decltype(every)::value;
+    if (s.groups == 2 && s.threads > 512) return f(mode, Two{}, Warp{}, every, integral_constant<int, 1024>{});
+    if (s.groups == 2 && (!kPairs || s.threads > 256))
+      return f(mode, Two{}, Warp{}, every, integral_constant<int, 512>{});
+    if constexpr (kPairs) {
+      if (s.groups == 2) return f(mode, Two{}, Warp{}, every, integral_constant<int, 256>{});
     }
+    if constexpr (!(kPairs && ESIZE == 4)) {
+      if (s.threads > 256) return f(mode, One{}, Warp{}, every, integral_constant<int, 512>{});
+    }
+    if constexpr (kAl) {
+      if (s.lanes == 16) return f(mode, One{}, integral_constant<int, 16>{}, every, integral_constant<int, 256>{});
+      if (s.lanes == 8) return f(mode, One{}, integral_constant<int, 8>{}, every, integral_constant<int, 256>{});
+    }
+    f(mode, One{}, Warp{}, every, integral_constant<int, 256>{});
   };
   auto with = [&](auto mode) { all ? go(mode, std::true_type{}) : go(mode, std::false_type{}); };
   if (s.mode == kAligned)
@@ -696,7 +697,7 @@ void residual_norm_fwd_launch(const ResidualNormArgs& a, const at::Tensor& y, co
     using T = decltype(t);
     const Shape s = shape_of(p, sizeof(T), false);
     const bool all = p.in[kH] != nullptr && p.n != nullptr && a.gate_kind != kGateFull;
-    with_shape(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
+    with_shape<sizeof(T), false>(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = kMaxT == 1024 ? 1 : 1024 / kMaxT;
       constexpr auto kernel =
           residual_norm_fwd<T, decltype(mode)::value, decltype(ng)::value, decltype(lanes)::value,
@@ -735,7 +736,7 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
     bool all = a.gate_kind != kGateFull;
     for (const void* q : {p.in[kH], p.in[kDy], p.in[kDn], (const void*)p.dx, (const void*)p.dh}) all = all && q != nullptr;
     const Shape s = shape_of(p, sizeof(T), all);
-    with_shape(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
+    with_shape<sizeof(T), true>(s, all, [&](auto mode, auto ng, auto lanes, auto every, auto maxt) {
       constexpr int kMaxT = decltype(maxt)::value, kMinB = decltype(ng)::value == 1 && kMaxT == 256 ? 2 : 1;
       constexpr auto kernel =
           residual_norm_bwd<T, decltype(mode)::value, decltype(ng)::value, decltype(lanes)::value,
