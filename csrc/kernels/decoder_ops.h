@@ -48,7 +48,8 @@ void residual_norm_bwd_launch(const ResidualNormArgs& a, const at::Tensor& rstd_
                               const at::Tensor& dgate, const at::Tensor& dpre, const at::Tensor& dpost);
 
 // Log probabilities of given tokens. logits [T, V] (last stride 1), tokens int64 [T].
-// stats fp32 [T, 2]: row maximum and log2 of the sum of exponentials; entropy, top_lp, top_ids may be undefined.
+// stats fp32 [T, 2]: a reference m, at most 8 / c below the row's maximum (c = log2(e) / temperature), and log2 of the sum
+// of the exponentials relative to it; entropy, top_lp, top_ids may be undefined.
 void token_logprobs_fwd_launch(const at::Tensor& logits, const at::Tensor& tokens, double inv_tau, int64_t top,
                                const at::Tensor& logprob, const at::Tensor& stats, const at::Tensor& entropy,
                                const at::Tensor& top_lp, const at::Tensor& top_ids);

@@ -9,9 +9,11 @@
 // positions before the values makes it slower: 117 us against 105 us without given positions, 119 us against 114 us
 // with them, for 32769 tokens of 40 heads x 128 bf16, where the copy's rate allows 103 us.)
 //
-// No table is read.  A frequency is a 64-bit fixed-point fraction of a revolution per position; times the position, modulo
-// 2^64, it is the angle without the whole revolutions, exact to |pos| 2^-65 of one (and 2^-53 of the angle from the
-// frequency itself).  So far positions lose nothing, no longest length has to be set, and no 64-bit floats are needed.
+// No table is read.  A frequency is a 64-bit fixed-point fraction of a revolution per position (cut off there); times the
+// position, modulo 2^64, it is the angle without the whole revolutions, exact to |pos| 2^-64 of one and to a few 2^-53 of the
+// angle from the frequency itself.  Its upper 32 bits, rounded to fp32, go on: 2^-26 of a revolution at worst, which is more
+// than the former up to positions of about 2^28.  So far positions lose nothing that fp32 would keep, no longest length has
+// to be set, and no 64-bit floats are needed.
 #include "decoder_ops.h"
 #include "vec.cuh"
 

@@ -19,8 +19,10 @@ dim at most 512; results are computed in fp32 and rounded once.  ``positions`` i
 int64 or int32, [tokens], [batch, tokens] or [1, tokens] ([batch] too, for one token
 per sequence); without it token i of a sequence has position ``offset + i`` (both
 together are refused).
-Positions are read on the device and may be any integer, negative ones included; an
-angle is as exact as its frequency in 64 bits (2^-53 of it).
+Positions are read on the device and may be any integer, negative ones included.  An
+angle is off by at most 2^-26 of a revolution (its rounding to fp32) and, from the
+64-bit frequency, a few 2^-53 of itself; up to positions of about 2^28 the latter is
+the smaller, beyond it grows with the position.
 
 A CUDA graph that records the backward must be the only holder of an autograd
 graph of its leaves: drop eager results of the same leaves before the capture.
