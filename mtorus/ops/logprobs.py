@@ -16,8 +16,10 @@ copied first), tokens int64 [...], top at most 64 and at most V.  Sums are held 
 * A token outside [0, V) is ignored: its logprob is 0 and has no gradient.  Entropy and
   alternatives of its row are computed all the same; where their gradients are absent or 0, the
   row's gradient is 0 whatever its logits are.
-* Masked logits (-inf, or the type's lowest value) have probability 0 unless the whole row is at
-  that value.  A row of -inf only: logprob -inf, entropy 0, no gradient.
+* Masked logits: -inf has probability 0; a row of -inf only has logprob -inf, entropy 0, no gradient.
+  The type's lowest value is a value like any other: its probability is 0 too unless the row's largest
+  is near it, measured in temperatures.  A row of nothing else is uniform; in fp16, where it is -65504,
+  it reaches 1e-30 at a temperature of 950.
 * Alternatives order by value, equal values by the lowest id.  Where fewer than ``top`` tokens are
   possible, impossible ones follow with logprob -inf.
 * Otherwise a row with a NaN or +inf has NaN results and gradients (its ids rank NaN with -inf).
