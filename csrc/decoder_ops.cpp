@@ -4,6 +4,8 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/util/ArrayRef.h>
+#include <c10/util/SmallVector.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -196,7 +198,7 @@ struct Term {
 
 // Whether `at` plus a multiple of each term's step (falling) can come within `width` of 0. Exact, but for a layout so
 // entangled that `budget` trials do not settle it: true.
-bool can_meet(const std::vector<Term>& terms, size_t next, int64_t at, int64_t width, int& budget) {
+bool can_meet(c10::ArrayRef<Term> terms, size_t next, int64_t at, int64_t width, int& budget) {
   if (next == terms.size()) return std::abs(at) < width;
   if (--budget < 0) return true;
   const Term& t = terms[next];
@@ -231,7 +233,7 @@ bool share_heads(const at::Tensor& q, const at::Tensor& k) {
   const int64_t between = reinterpret_cast<intptr_t>(k.data_ptr()) - reinterpret_cast<intptr_t>(q.data_ptr());
   if (between >= extent(q) || -between >= extent(k)) return false;
   // a head of k lies `between` + its own steps - those of the head of q from that
-  std::vector<Term> terms;
+  c10::SmallVector<Term, 6> terms;
   for (int sign : {-1, 1}) {
     const at::Tensor& t = sign < 0 ? q : k;
     for (int64_t i = 0; i < t.dim() - 1; ++i) {
@@ -249,7 +251,7 @@ bool share_heads(const at::Tensor& q, const at::Tensor& k) {
 
 // Whether the heads of x are known to lie apart from one another: each axis steps over all that the smaller ones cover.
 bool heads_apart(const at::Tensor& x) {
-  std::vector<std::pair<int64_t, int64_t>> axes;
+  c10::SmallVector<std::pair<int64_t, int64_t>, 4> axes;
   for (int64_t i = 0; i < x.dim(); ++i) {
     if (x.size(i) > 1) axes.emplace_back(x.stride(i), x.size(i));
   }
@@ -315,17 +317,20 @@ void rotary_inplace(at::Tensor q, const OptTensor& k, const at::Tensor& turns, i
     TORCH_CHECK(!needs_grad({t}),
                 "rotary_: works in place and records no gradient; use rotary() on tensors that require one");
     TORCH_CHECK_VALUE(t->size(-1) <= 1 || t->stride(-1) == 1, "rotary_: the head dim must have stride 1");
-    at::assert_no_internal_overlap(*t);
-    TORCH_CHECK_VALUE(t->numel() == 0 || heads_apart(*t), "rotary_: ", t == &q ? "q" : "k",
-                      " has heads that are the same memory in some of their values (sizes ", t->sizes(), ", strides ",
-                      t->strides(), ")");
+    if (t->numel() > 0 && !heads_apart(*t)) {
+      at::assert_no_internal_overlap(*t);
+      TORCH_CHECK_VALUE(false, "rotary_: ", t == &q ? "q" : "k", " has heads that are the same memory in some of their ",
+                        "values (sizes ", t->sizes(), ", strides ", t->strides(), ")");
+    }
   }
   if (kt.defined()) {
     check_pair(q, kt);
     TORCH_CHECK_VALUE(q.data_ptr() != kt.data_ptr() || q.numel() == 0, "rotary_: q and k are the same memory");
-    at::assert_no_overlap(q, kt);
-    TORCH_CHECK_VALUE(!share_heads(q, kt), "rotary_: q and k are the same memory in some of their heads, or in a layout ",
-                      "too entangled to tell (strides ", q.strides(), " and ", kt.strides(), ")");
+    if (share_heads(q, kt)) {
+      at::assert_no_overlap(q, kt);
+      TORCH_CHECK_VALUE(false, "rotary_: q and k are the same memory in some of their heads, or in a layout too entangled ",
+                        "to tell (strides ", q.strides(), " and ", kt.strides(), ")");
+    }
   }
   const at::Tensor qt = tokens_of(q);
   const OptTensor pos = positions_of(positions, qt.size(0), qt.size(1), offset);
